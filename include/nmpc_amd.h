@@ -265,6 +265,35 @@ int nmpc_target_select_state_ws(const nmpc_model* m, int nb, int nsamp, const do
                                 int max_lpv, double tol, double* Xs, double* Us, double* Es, int* iters,
                                 int* status, void* workspace, unsigned long long workspace_bytes, void* stream);
 
+/* ---- operators of sequence models: layers of learned models that read whole records of samples (no counterpart in the
+ * reference; nmpc_lpv_scan is the linear parameter-varying recurrence x+ = A(p) x + B(p) u of nmpc_lpv_rk4 / nmpc_condense
+ * with a diagonal A and the input as scheduling variable, over records of any length).
+ * Element types of samples and their gradients: NMPC_F32 / NMPC_BF16 / NMPC_F16; parameters of the filter and the
+ * recurrence, their gradients and states are fp32.  All sums are fp32 and joined in a fixed order: results do not change
+ * from call to call.  nb sequences of L steps and D channels; samples are [nb][L][D] with channels contiguous and the
+ * strides of sequence and step given in elements (_bs, _ts; parts of a wider tensor need no copy), outputs are contiguous.
+ * lengths[nb] (device int32, may be NULL; clamped to 0..L): steps from lengths[b] on are not read, their outputs and
+ * gradients are zero, and final states are those after step lengths[b] - 1. */
+enum { NMPC_F32 = 0, NMPC_BF16 = 1, NMPC_F16 = 2 };
+enum { NMPC_ACT_NONE = 0, NMPC_ACT_SILU = 1, NMPC_ACT_GELU = 2, NMPC_ACT_TANH = 3, NMPC_ACT_SIGMOID = 4 };
+
+/* Causal convolution, one filter of W <= 8 taps per channel, act = none or SiLU:
+ *   line = [start; u],  y[t,c] = act(bias[c] + sum_j w[c,j] line[t+j,c]).
+ * w[D,W], bias[D] (fp32, may be NULL); start[nb,W-1,D]: the samples before the first, oldest first (NULL = zeros);
+ * window[nb,W-1,D] (may be NULL): the last W-1 rows of the line, the start of what follows.
+ * _bwd: dy like y (strided), dwindow (may be NULL) -> du, dw[D,W], dbias[D] (may be NULL), dstart (may be NULL); workspace:
+ * nmpc_causal_conv_workspace_bytes, contents need not be preserved.
+ * _step: one sample u[nb,D] of every sequence; window is read and moved on by one row in place. */
+int nmpc_causal_conv(int dtype, int nb, int L, int D, int W, const void* u, long long u_bs, long long u_ts, const float* w,
+                     const float* bias, int act, const void* start, const int* lengths, void* y, void* window, void* stream);
+unsigned long long nmpc_causal_conv_workspace_bytes(int nb, int L, int D, int W);
+int nmpc_causal_conv_bwd(int dtype, int nb, int L, int D, int W, const void* u, long long u_bs, long long u_ts, const float* w,
+                         const float* bias, int act, const void* start, const int* lengths, const void* dy, long long dy_bs,
+                         long long dy_ts, const void* dwindow, void* du, float* dw, float* dbias, void* dstart,
+                         void* workspace, unsigned long long workspace_bytes, void* stream);
+int nmpc_causal_conv_step(int dtype, int nb, int D, int W, void* window, const void* u, long long u_bs, const float* w,
+                          const float* bias, int act, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,14 @@ SIGNATURES = {
     "nmpc_ctrl_stats": (ctypes.c_int, [c_void_p, ctypes.POINTER(ctypes.c_longlong), c_void_p]),
     "nmpc_ctrl_set_status_log": (ctypes.c_int, [c_void_p, c_void_p]),
     "nmpc_ctrl_set_embed_stamps": (ctypes.c_int, [c_void_p, c_void_p, ctypes.c_int]),
+    "nmpc_causal_conv": (ctypes.c_int, [ctypes.c_int] * 5 + [c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_void_p, c_void_p,
+                                        ctypes.c_int] + [c_void_p] * 5),
+    "nmpc_causal_conv_workspace_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 4),
+    "nmpc_causal_conv_bwd": (ctypes.c_int, [ctypes.c_int] * 5 + [c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_void_p, c_void_p,
+                                            ctypes.c_int, c_void_p, c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_longlong] +
+                             [c_void_p] * 6 + [ctypes.c_ulonglong, c_void_p]),
+    "nmpc_causal_conv_step": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p,
+                                             ctypes.c_int, c_void_p, c_void_p]),
 }
 
 MAX_NODES = 256

@@ -1,0 +1,205 @@
+"""Operators of sequence models on the GPU: causal convolution, selective LPV scan, gated feed-forward projections.
+
+Each whole-sequence operator comes in three forms: `op(...)` (differentiable through torch.autograd where an input asks for
+it), and the pair `op_fwd(...)` -> outputs and what the gradient needs, `op_bwd(saved, gradients of the outputs)` -> the
+gradients, which records no autograd graph and can be captured into a HIP graph.  `*_step` is the form for one sample of
+every running sequence and moves its state on in place.
+
+Samples are [batch, steps, channels] (channels contiguous; other layouts are copied) in float32, bfloat16 or float16;
+states of the scan and all sums are fp32.  `lengths` [batch] (integers, on the GPU): steps from lengths[b] on are padding -
+they are not read, and their outputs and gradients are zero."""
+import torch
+
+from . import _lib
+from ._lib import NmpcError, lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "tanh": 3, "sigmoid": 4}
+
+
+def _need(ok, what, text, *args):
+    if not ok:
+        raise NmpcError("%s: %s" % (what, text % args if args else text))
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(dev, what, fn, *args):
+    """fn(*args, current stream of dev) with dev current; an error becomes NmpcError."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, what)
+
+
+def _on_gpu(what, x, *others):
+    """All tensors on x's GPU (checked last, after the shapes)."""
+    _lib.require_gpu()
+    _need(x.is_cuda, what, "tensors must be on the GPU, got %s", x.device)
+    for t in others:
+        _need(t is None or t.device == x.device, what, "tensors on different devices: %s and %s", x.device, getattr(t, "device", None))
+
+
+def _samples(what, name, t, shape, dtype):
+    """A sample tensor of this shape and type with contiguous channels (a copy only where they are not)."""
+    _need(torch.is_tensor(t) and tuple(t.shape) == tuple(shape), what, "%s must be %s, got %s", name, list(shape),
+          list(t.shape) if torch.is_tensor(t) else type(t).__name__)
+    _need(t.dtype == dtype, what, "%s is %s, the samples are %s", name, t.dtype, dtype)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _param(what, name, t, shape):
+    """A parameter as contiguous fp32."""
+    _need(torch.is_tensor(t) and tuple(t.shape) == tuple(shape), what, "%s must be %s, got %s", name, list(shape),
+          list(t.shape) if torch.is_tensor(t) else type(t).__name__)
+    _need(t.is_floating_point(), what, "%s is %s, expected floating point", name, t.dtype)
+    t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
+def _lengths(what, t, nb):
+    if t is None:
+        return None
+    _need(torch.is_tensor(t) and t.dim() == 1 and t.shape[0] == nb, what, "lengths must be [%d]", nb)
+    _need(not t.is_floating_point() and not t.is_complex() and t.dtype != torch.bool, what, "lengths are %s, expected integers", t.dtype)
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _records(what, *tensors):
+    """Does this call have to be recorded by autograd?  Under graph capture it is refused: autograd's own bookkeeping of
+    leaves that an eager graph still holds cannot be captured."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    _need(not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()), what,
+          "autograd is not recorded under graph capture; capture the pair %s_fwd / %s_bwd (or call under torch.no_grad())", what, what)
+    return True
+
+
+class Saved:
+    """What a forward pass leaves for its gradient: `tensors` and plain values."""
+
+    __slots__ = ("what", "tensors", "values")
+
+    def __init__(self, what, tensors, values):
+        self.what, self.tensors, self.values = what, tensors, values
+
+
+def _saved(what, saved):
+    _need(isinstance(saved, Saved) and saved.what == what, what + "_bwd", "expects what %s_fwd returned last", what)
+    return saved.tensors, saved.values
+
+
+class _Recorded(torch.autograd.Function):
+    """An operator's pair as one node of an autograd graph.  fwd() -> (outputs tuple, Saved); bwd(saved, *gradients) ->
+    gradients in the order of `inputs`."""
+
+    @staticmethod
+    def forward(ctx, fwd, bwd, *inputs):
+        outs, saved = fwd()
+        ctx.save_for_backward(*saved.tensors)
+        ctx.what, ctx.values, ctx.bwd = saved.what, saved.values, bwd
+        ctx.set_materialize_grads(False)
+        return outs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        return (None, None) + tuple(ctx.bwd(Saved(ctx.what, ctx.saved_tensors, ctx.values), *grads))
+
+
+# ---- causal convolution ---------------------------------------------------------------------------------------------
+def _conv_args(what, u, w, bias, act, start, lengths, steps=True):
+    _need(torch.is_tensor(u) and u.dim() == (3 if steps else 2), what, "u must be %s", "[batch, steps, channels]" if steps else "[batch, channels]")
+    _need(u.dtype in _DTYPES, what, "samples are %s, expected float32, bfloat16 or float16", u.dtype)
+    _need(torch.is_tensor(w) and w.dim() == 2 and 1 <= w.shape[1] <= 8, what, "w must be [channels, taps] with 1..8 taps")
+    _need(act in (None, "none", "silu"), what, "activation %r (None or 'silu')", act)
+    nb, d, taps = u.shape[0], u.shape[-1], w.shape[1]
+    _need(d >= 1, what, "no channels")
+    w = _param(what, "w", w, (d, taps))
+    bias = None if bias is None else _param(what, "bias", bias, (d,))
+    if start is not None:
+        _need(steps or not torch.is_tensor(start) or start.is_contiguous(), what, "window must be a contiguous tensor: it is moved on in place")
+        start = _samples(what, "start" if steps else "window", start, (nb, taps - 1, d), u.dtype).contiguous()
+    u = u if u.stride(-1) == 1 or d == 1 else u.contiguous()
+    return u, w, bias, start, _lengths(what, lengths, nb)
+
+
+def _conv_fwd(what, u, w, bias, act, start, lengths, want_window):
+    u, w, bias, start, lengths = _conv_args(what, u, w, bias, act, start, lengths)
+    _on_gpu(what, u, w, bias, start, lengths)
+    nb, steps, d = u.shape
+    y = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
+    window = torch.empty((nb, w.shape[1] - 1, d), dtype=u.dtype, device=u.device) if want_window else None
+    _call(u.device, what, lib().nmpc_causal_conv, _DTYPES[u.dtype], nb, steps, d, w.shape[1], _p(u), u.stride(0), u.stride(1), _p(w),
+          _p(bias), _ACTS[act], _p(start), _p(lengths), _p(y), _p(window))
+    return y, window, (u, w, bias, start, lengths)
+
+
+def causal_conv_fwd(u, w, bias=None, act=None, start=None, lengths=None):
+    """causal_conv that keeps what its gradient needs: (y, window, saved)."""
+    with torch.no_grad():
+        y, window, tensors = _conv_fwd("causal_conv_fwd", u, w, bias, act, start, lengths, True)
+    return y, window, Saved("causal_conv", tensors, (act,))
+
+
+def causal_conv_bwd(saved, dy, dwindow=None):
+    """Gradients of causal_conv_fwd's call: {"du", "dw", "dbias", "dstart"} (dw and dbias fp32; None for inputs that were
+    not given).  dy [batch, steps, channels] and dwindow [batch, taps-1, channels] (None = zero): gradients of y and window."""
+    what = "causal_conv_bwd"
+    (u, w, bias, start, lengths), (act,) = _saved("causal_conv", saved)
+    nb, steps, d = u.shape
+    taps = w.shape[1]
+    dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
+    dwindow = None if dwindow is None else _samples(what, "dwindow", dwindow, (nb, taps - 1, d), u.dtype).contiguous()
+    _on_gpu(what, u, dy, dwindow)
+    du = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
+    dw = torch.empty_like(w)
+    dbias = None if bias is None else torch.empty_like(bias)
+    dstart = None if start is None else torch.empty_like(start)
+    size = lib().nmpc_causal_conv_workspace_bytes(nb, steps, d, taps)
+    work = torch.empty(size, dtype=torch.uint8, device=u.device)
+    _call(u.device, what, lib().nmpc_causal_conv_bwd, _DTYPES[u.dtype], nb, steps, d, taps, _p(u), u.stride(0), u.stride(1), _p(w),
+          _p(bias), _ACTS[act], _p(start), _p(lengths), _p(dy), dy.stride(0), dy.stride(1), _p(dwindow), _p(du), _p(dw), _p(dbias),
+          _p(dstart), _p(work), size)
+    return {"du": du, "dw": dw, "dbias": dbias, "dstart": dstart}
+
+
+def causal_conv(u, w, bias=None, act=None, start=None, lengths=None, return_state=False):
+    """y[b,t,c] = act(bias[c] + sum_j w[c,j] line[b,t+j,c]),  line = [start; u] along time.
+
+    u [batch, steps, channels]; w [channels, taps], 1..8 taps; bias [channels]; act None or "silu"; start [batch, taps-1,
+    channels]: the samples before the first, oldest first (None = zeros).  Returns y, with return_state also the window
+    [batch, taps-1, channels] of the last samples: the start of what follows, and causal_conv_step's state."""
+    what = "causal_conv"
+    if not _records(what, u, w, bias, start):
+        with torch.no_grad():
+            y, window, _ = _conv_fwd(what, u, w, bias, act, start, lengths, return_state)
+        return (y, window) if return_state else y
+
+    def fwd():
+        y, window, saved = causal_conv_fwd(u, w, bias, act, start, lengths)
+        return (y, window), saved
+
+    def bwd(saved, dy, dwindow):
+        g = causal_conv_bwd(saved, dy, dwindow)
+        return (g["du"], g["dw"].to(w.dtype), None if bias is None else g["dbias"].to(bias.dtype), g["dstart"])
+    y, window = _Recorded.apply(fwd, bwd, u, w, bias, start)
+    return (y, window) if return_state else y
+
+
+def causal_conv_step(window, u, w, bias=None, act=None):
+    """One sample u [batch, channels] of every sequence: returns y [batch, channels] and moves window [batch, taps-1,
+    channels] (contiguous) on by one row in place."""
+    what = "causal_conv_step"
+    _need(not _records(what, window, u, w, bias), what, "works in place and has no gradient; use causal_conv")
+    u, w, bias, window, _ = _conv_args(what, u, w, bias, act, window, None, steps=False)
+    _need(window is not None, what, "needs a window")
+    _on_gpu(what, u, w, bias, window)
+    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    _call(u.device, what, lib().nmpc_causal_conv_step, _DTYPES[u.dtype], u.shape[0], u.shape[1], w.shape[1], _p(window), _p(u),
+          u.stride(0), _p(w), _p(bias), _ACTS[act], _p(y))
+    return y

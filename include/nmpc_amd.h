@@ -294,6 +294,43 @@ int nmpc_causal_conv_bwd(int dtype, int nb, int L, int D, int W, const void* u, 
 int nmpc_causal_conv_step(int dtype, int nb, int D, int W, void* window, const void* u, long long u_bs, const float* w,
                           const float* bias, int act, void* y, void* stream);
 
+/* Selective state-space scan: the diagonal LPV recurrence, per channel d with N <= 64 states,
+ *   delta = softplus(dt + dt_bias)  (softplus = 0: dt + dt_bias),
+ *   x_t = exp(delta A) x_{t-1} + delta B_t u_t,   y_t = (C_t . x_t + D u_t) silu(z_t).
+ * B and C are shared by the D / G neighbouring channels of a group: [nb][L][G][N], (G, N) contiguous.  A[D,N], D_skip[D],
+ * dt_bias[D], start / last[nb,D,N] (states) are fp32; D_skip, z, dt_bias, start, last may be NULL.
+ * nmpc_lpv_scan: -> y, last; saved (NULL = no gradient wanted): nmpc_lpv_scan_saved_bytes of device memory that
+ * nmpc_lpv_scan_bwd reads.
+ * nmpc_lpv_scan_bwd: the same inputs and saved, dy (strided like y), dlast (NULL = zero) -> du, ddt, dz, dB, dC (samples,
+ * contiguous), dA, dD, ddt_bias, dstart (fp32; dstart may be NULL).
+ * nmpc_lpv_scan_step: one sample of every sequence, u / dt / z [nb][D], B / C [nb][G][N] (_ts unused); `last` is the state,
+ * read and replaced.
+ * workspace: nmpc_lpv_scan_workspace_bytes (0 for some sizes), contents need not be preserved; calls that overlap in time
+ * need one each. */
+typedef struct nmpc_scan_args {
+    int struct_size;                     /* sizeof(nmpc_scan_args) of the caller's header; checked */
+    int dtype, nb, L, D, N, G, softplus;
+    const void *u, *dt, *B, *C, *z;
+    long long u_bs, u_ts, dt_bs, dt_ts, B_bs, B_ts, C_bs, C_ts, z_bs, z_ts;
+    const float *A, *D_skip, *dt_bias, *start;
+    const int* lengths;
+    void* y;
+    float* last;
+    void* saved;
+    const void* dy;
+    long long dy_bs, dy_ts;
+    const float* dlast;
+    void *du, *ddt, *dB, *dC, *dz;
+    float *dA, *dD, *ddt_bias, *dstart;
+    void* workspace;
+    unsigned long long workspace_bytes;
+} nmpc_scan_args;
+unsigned long long nmpc_lpv_scan_saved_bytes(int nb, int L, int D, int N);
+unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D, int N, int G, int backward);
+int nmpc_lpv_scan(const nmpc_scan_args* args, void* stream);
+int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream);
+int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

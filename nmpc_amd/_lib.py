@@ -74,6 +74,11 @@ SIGNATURES = {
                              [c_void_p] * 6 + [ctypes.c_ulonglong, c_void_p]),
     "nmpc_causal_conv_step": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p, c_void_p, ctypes.c_longlong, c_void_p, c_void_p,
                                              ctypes.c_int, c_void_p, c_void_p]),
+    "nmpc_lpv_scan_saved_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 4),
+    "nmpc_lpv_scan_workspace_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 6),
+    "nmpc_lpv_scan": (ctypes.c_int, [c_void_p, c_void_p]),
+    "nmpc_lpv_scan_bwd": (ctypes.c_int, [c_void_p, c_void_p]),
+    "nmpc_lpv_scan_step": (ctypes.c_int, [c_void_p, c_void_p]),
 }
 
 MAX_NODES = 256
@@ -98,6 +103,17 @@ class CtrlConfig(ctypes.Structure):
     def __init__(self, *a, **k):
         super().__init__(*a, **k)
         self.struct_size = ctypes.sizeof(CtrlConfig)
+
+
+class ScanArgs(ctypes.Structure):
+    """struct nmpc_scan_args of include/nmpc_amd.h"""
+    _fields_ = ([(n, ctypes.c_int) for n in ("struct_size", "dtype", "nb", "L", "D", "N", "G", "softplus")] +
+                [(n, c_void_p) for n in ("u", "dt", "B", "C", "z")] +
+                [(n, ctypes.c_longlong) for n in ("u_bs", "u_ts", "dt_bs", "dt_ts", "B_bs", "B_ts", "C_bs", "C_ts", "z_bs", "z_ts")] +
+                [(n, c_void_p) for n in ("A", "D_skip", "dt_bias", "start", "lengths", "y", "last", "saved", "dy")] +
+                [("dy_bs", ctypes.c_longlong), ("dy_ts", ctypes.c_longlong)] +
+                [(n, c_void_p) for n in ("dlast", "du", "ddt", "dB", "dC", "dz", "dA", "dD", "ddt_bias", "dstart", "workspace")] +
+                [("workspace_bytes", ctypes.c_ulonglong)])
 
 
 _lib = None

@@ -8,6 +8,8 @@ every running sequence and moves its state on in place.
 Samples are [batch, steps, channels] (channels contiguous; other layouts are copied) in float32, bfloat16 or float16;
 states of the scan and all sums are fp32.  `lengths` [batch] (integers, on the GPU): steps from lengths[b] on are padding -
 they are not read, and their outputs and gradients are zero."""
+import ctypes
+
 import torch
 
 from . import _lib
@@ -72,7 +74,7 @@ def _lengths(what, t, nb):
 def _records(what, *tensors):
     """Does this call have to be recorded by autograd?  Under graph capture it is refused: autograd's own bookkeeping of
     leaves that an eager graph still holds cannot be captured."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled() or not any(torch.is_tensor(t) and t.requires_grad for t in tensors):
         return False
     _need(not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()), what,
           "autograd is not recorded under graph capture; capture the pair %s_fwd / %s_bwd (or call under torch.no_grad())", what, what)
@@ -202,4 +204,155 @@ def causal_conv_step(window, u, w, bias=None, act=None):
     y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
     _call(u.device, what, lib().nmpc_causal_conv_step, _DTYPES[u.dtype], u.shape[0], u.shape[1], w.shape[1], _p(window), _p(u),
           u.stride(0), _p(w), _p(bias), _ACTS[act], _p(y))
+    return y
+
+
+# ---- selective LPV scan ---------------------------------------------------------------------------------------------
+def _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, steps=True):
+    lead = 2 if steps else 1
+    _need(torch.is_tensor(u) and u.dim() == lead + 1, what, "u must be %s", "[batch, steps, channels]" if steps else "[batch, channels]")
+    _need(u.dtype in _DTYPES, what, "samples are %s, expected float32, bfloat16 or float16", u.dtype)
+    d = u.shape[-1]
+    _need(torch.is_tensor(A) and A.dim() == 2 and A.shape[0] == d and 1 <= A.shape[1] <= 64, what, "A must be [channels, states] with 1..64 states")
+    n = A.shape[1]
+    _need(torch.is_tensor(B) and B.dim() == lead + 2 and B.shape[:lead] == u.shape[:lead] and B.shape[-1] == n, what,
+          "B must be %s", list(u.shape[:lead]) + ["groups", n])
+    groups = B.shape[-2]
+    _need(d >= 1 and groups >= 1 and d % groups == 0, what, "%d groups do not divide %d channels", groups, d)
+    u = u if u.stride(-1) == 1 or d == 1 else u.contiguous()
+    dt = _samples(what, "dt", dt, u.shape, u.dtype)
+    z = None if z is None else _samples(what, "z", z, u.shape, u.dtype)
+
+    def shared(name, t):
+        t = _samples(what, name, t, tuple(u.shape[:lead]) + (groups, n), u.dtype)
+        return t if groups == 1 or t.stride(-2) == n else t.contiguous()
+    return (u, dt, _param(what, "A", A, (d, n)), shared("B", B), shared("C", C), None if D is None else _param(what, "D", D, (d,)), z,
+            None if dt_bias is None else _param(what, "dt_bias", dt_bias, (d,)))
+
+
+def _scan_struct(u, dt, A, B, C, D, z, dt_bias, softplus):
+    """The argument struct with the inputs filled in; unused strides of single steps stay zero."""
+    s = _lib.ScanArgs()
+    s.struct_size, s.dtype, s.nb, s.D, s.softplus = ctypes.sizeof(_lib.ScanArgs), _DTYPES[u.dtype], u.shape[0], u.shape[-1], int(bool(softplus))
+    s.N, s.G = A.shape[1], B.shape[-2]
+    s.u, s.dt, s.A, s.B, s.C = u.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr()
+    s.u_bs, s.dt_bs, s.B_bs, s.C_bs = u.stride(0), dt.stride(0), B.stride(0), C.stride(0)
+    if D is not None:
+        s.D_skip = D.data_ptr()
+    if dt_bias is not None:
+        s.dt_bias = dt_bias.data_ptr()
+    if z is not None:
+        s.z, s.z_bs = z.data_ptr(), z.stride(0)
+    if u.dim() == 3:
+        s.L, s.u_ts, s.dt_ts, s.B_ts, s.C_ts = u.shape[1], u.stride(1), dt.stride(1), B.stride(1), C.stride(1)
+        if z is not None:
+            s.z_ts = z.stride(1)
+    else:
+        s.L = 1
+    return s
+
+
+def _states(what, name, t, nb, A):
+    if t is None:
+        return None
+    _need(torch.is_tensor(t) and tuple(t.shape) == (nb,) + tuple(A.shape), what, "%s must be %s", name, [nb] + list(A.shape))
+    _need(t.dtype == torch.float32, what, "%s is %s, states are float32", name, t.dtype)
+    return t.contiguous()
+
+
+def _scan_work(s, dev, backward):
+    size = lib().nmpc_lpv_scan_workspace_bytes(s.nb, s.L, s.D, s.N, s.G, backward)
+    if not size:
+        return None
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    s.workspace, s.workspace_bytes = work.data_ptr(), size
+    return work
+
+
+def _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, want_state, want_saved):
+    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias)
+    nb, steps, d = u.shape
+    start, lengths = _states(what, "start", start, nb, A), _lengths(what, lengths, nb)
+    _on_gpu(what, *tensors, start, lengths)
+    s = _scan_struct(*tensors, softplus)
+    s.start, s.lengths = _p(start), _p(lengths)
+    y = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
+    last = torch.empty((nb, d, A.shape[1]), dtype=torch.float32, device=u.device) if want_state else None
+    saved = None
+    if want_saved:
+        saved = torch.empty(lib().nmpc_lpv_scan_saved_bytes(nb, steps, d, A.shape[1]), dtype=torch.uint8, device=u.device)
+    s.y, s.last, s.saved = y.data_ptr(), _p(last), _p(saved)
+    work = _scan_work(s, u.device, 0)  # noqa: F841  (held until the launch)
+    _call(u.device, what, lib().nmpc_lpv_scan, ctypes.addressof(s))
+    return y, last, tensors + (start, lengths, saved)
+
+
+def lpv_scan_fwd(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, start=None, lengths=None):
+    """lpv_scan that keeps what its gradient needs: (y, last, saved).  Besides the inputs that is the state before every
+    32nd step."""
+    with torch.no_grad():
+        y, last, tensors = _scan_fwd("lpv_scan_fwd", u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, True, True)
+    return y, last, Saved("lpv_scan", tensors, (bool(softplus),))
+
+
+def lpv_scan_bwd(saved, dy, dlast=None):
+    """Gradients of lpv_scan_fwd's call: {"du", "ddt", "dA", "dB", "dC", "dD", "dz", "ddt_bias", "dstart"}, those of samples
+    in the samples' type, the others fp32; None for inputs that were not given.  dy [batch, steps, channels] and dlast
+    [batch, channels, states] (None = zero): gradients of y and of the last state."""
+    what = "lpv_scan_bwd"
+    (u, dt, A, B, C, D, z, dt_bias, start, lengths, kept), (softplus,) = _saved("lpv_scan", saved)
+    dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
+    dlast = _states(what, "dlast", dlast, u.shape[0], A)
+    _on_gpu(what, u, dy, dlast)
+    s = _scan_struct(u, dt, A, B, C, D, z, dt_bias, softplus)
+    s.lengths, s.saved, s.dy, s.dy_bs, s.dy_ts, s.dlast = _p(lengths), _p(kept), dy.data_ptr(), dy.stride(0), dy.stride(1), _p(dlast)
+    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    g = {"du": like(u), "ddt": like(dt), "dA": like(A), "dB": like(B), "dC": like(C), "dD": like(D), "dz": like(z),
+         "ddt_bias": like(dt_bias), "dstart": like(start)}
+    for name, t in g.items():
+        setattr(s, name, _p(t))
+    work = _scan_work(s, u.device, 1)  # noqa: F841  (held until the launch)
+    _call(u.device, what, lib().nmpc_lpv_scan_bwd, ctypes.addressof(s))
+    return g
+
+
+def lpv_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, start=None, lengths=None, return_state=False):
+    """Selective state-space scan, the diagonal LPV recurrence over a record:
+        delta = softplus(dt + dt_bias)   (softplus=False: dt + dt_bias),
+        x_t = exp(delta A) x_{t-1} + delta B_t u_t,    y_t = (C_t . x_t + D u_t) silu(z_t).
+
+    u, dt, z [batch, steps, channels]; A [channels, states], 1..64 states; B, C [batch, steps, groups, states], shared by the
+    channels / groups neighbouring channels of a group; D, dt_bias [channels]; start [batch, channels, states] fp32 (None =
+    zeros).  Returns y, with return_state also the state after the last step, lpv_scan_step's state."""
+    what = "lpv_scan"
+    if not _records(what, u, dt, A, B, C, D, z, dt_bias, start):
+        with torch.no_grad():
+            y, last, _ = _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, return_state, False)
+        return (y, last) if return_state else y
+
+    def fwd():
+        y, last, saved = lpv_scan_fwd(u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths)
+        return (y, last), saved
+
+    def bwd(saved, dy, dlast):
+        g = lpv_scan_bwd(saved, dy, dlast)
+        return (g["du"], g["ddt"], g["dA"].to(A.dtype), g["dB"], g["dC"], None if D is None else g["dD"].to(D.dtype), g["dz"],
+                None if dt_bias is None else g["ddt_bias"].to(dt_bias.dtype), g["dstart"])
+    y, last = _Recorded.apply(fwd, bwd, u, dt, A, B, C, D, z, dt_bias, start)
+    return (y, last) if return_state else y
+
+
+def lpv_scan_step(state, u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True):
+    """One sample of every sequence: u, dt, z [batch, channels], B, C [batch, groups, states].  Returns y [batch, channels];
+    state [batch, channels, states] (fp32, contiguous) moves on by one step in place."""
+    what = "lpv_scan_step"
+    _need(not _records(what, state, u, dt, A, B, C, D, z, dt_bias), what, "works in place and has no gradient; use lpv_scan")
+    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, steps=False)
+    _need(torch.is_tensor(state) and state.is_contiguous(), what, "state must be a contiguous tensor: it is moved on in place")
+    state = _states(what, "state", state, u.shape[0], A)
+    _on_gpu(what, *tensors, state)
+    s = _scan_struct(*tensors, softplus)
+    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    s.y, s.last = y.data_ptr(), state.data_ptr()
+    _call(u.device, what, lib().nmpc_lpv_scan_step, ctypes.addressof(s))
     return y

@@ -28,16 +28,16 @@ def leaf(t):
     return None if t is None else t.detach().cpu().double().requires_grad_()
 
 
-def assert_close(got, want, roundings, scale, name):
+def assert_close(got, want, roundings, scale, name, floor=0.0):
     """|got - want| <= half a step of got's type (one rounding at the end) + `roundings` roundings to fp32 of terms whose
-    magnitudes add up to `scale` (a tensor or number)."""
+    magnitudes add up to `scale` (a tensor or number), plus `floor` where values leave fp32's normal range."""
     half = torch.finfo(got.dtype).eps / 2
     got64, want = f64(got), f64(want)
     assert got64.shape == want.shape, (name, got64.shape, want.shape)
     slack = roundings * U32 * (scale if torch.is_tensor(scale) else torch.tensor(float(scale), dtype=torch.float64))
     smallest = torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps
     # the final rounding acts on the fp32 value, which is off by the slack itself
-    tol = half * (want.abs() + slack) + slack + smallest
+    tol = half * (want.abs() + slack) + slack + smallest + floor
     off = (got64 - want).abs()
     bad = ~(off <= tol)
     assert not bad.any(), "%s: %d of %d outside; worst %.3g times its bound (got %r, want %r)" % (

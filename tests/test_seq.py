@@ -69,3 +69,76 @@ def test_seq_operators_need_a_gpu():
         pytest.skip("GPU present")
     with pytest.raises(nmpc_amd.NmpcError):
         nmpc_amd.causal_conv(torch.zeros(1, 4, 8), torch.zeros(8, 4))
+
+
+def test_oracle_scan_gradient_against_differences():
+    g = rng(2)
+    nb, steps, d, n, groups = 2, 4, 4, 2, 2
+    leaves = [_double(g, nb, steps, d), _double(g, nb, steps, d), (-torch.rand(d, n, generator=g, dtype=torch.float64)).requires_grad_(),
+              _double(g, nb, steps, groups, n), _double(g, nb, steps, groups, n), _double(g, d), _double(g, nb, steps, d), _double(g, d),
+              _double(g, nb, d, n)]
+    for lengths in (None, [3, 0]):
+        assert torch.autograd.gradcheck(lambda *a: oracle.lpv_scan(*a[:8], start=a[8], lengths=lengths), leaves)
+
+
+def test_scan_refusals():
+    u, A, B = torch.zeros(2, 6, 8), torch.zeros(8, 4), torch.zeros(2, 6, 2, 4)
+    ok = dict(u=u, dt=u, A=A, B=B, C=B)
+    bad = [
+        (dict(u=u[0]), "batch, steps, channels"), (dict(u=u.double()), "float32, bfloat16"), (dict(dt=u[:, :5]), "dt must be"),
+        (dict(dt=u.half()), "the samples are"), (dict(A=torch.zeros(8, 65)), "1..64 states"), (dict(A=torch.zeros(7, 4)), "A must be"),
+        (dict(B=torch.zeros(2, 6, 3, 4), C=torch.zeros(2, 6, 3, 4)), "do not divide"), (dict(B=torch.zeros(2, 6, 4)), "B must be"),
+        (dict(C=torch.zeros(2, 6, 1, 4)), "C must be"), (dict(D=torch.zeros(4)), "D must be"), (dict(z=u[..., :4]), "z must be"),
+        (dict(dt_bias=torch.zeros(8, 1)), "dt_bias must be"), (dict(start=torch.zeros(2, 8, 5)), "start must be"),
+        (dict(start=torch.zeros(2, 8, 4).half()), "states are float32"), (dict(lengths=torch.zeros(2)), "integers"),
+    ]
+    for change, text in bad:
+        for fn in (nmpc_amd.lpv_scan, nmpc_amd.lpv_scan_fwd):
+            with pytest.raises(nmpc_amd.NmpcError, match=text):
+                fn(**{**ok, **change})
+    one = dict(u=u[:, 0], dt=u[:, 0], A=A, B=B[:, 0], C=B[:, 0])
+    for state, text in ((torch.zeros(2, 8, 5), "state must be"), (torch.zeros(2, 8, 4).bfloat16(), "states are float32"),
+                        (torch.zeros(2, 4, 8).transpose(1, 2), "contiguous")):
+        with pytest.raises(nmpc_amd.NmpcError, match=text):
+            nmpc_amd.lpv_scan_step(state, **one)
+    with pytest.raises(nmpc_amd.NmpcError, match="no gradient"):
+        nmpc_amd.lpv_scan_step(torch.zeros(2, 8, 4), **{**one, "A": A.clone().requires_grad_()})
+
+
+def test_scan_abi(tmp_path):
+    """The ctypes mirror has the header's layout; every refusal comes back before anything is launched."""
+    import os
+    import subprocess
+    from conftest import ROOT
+    src, exe = tmp_path / "sz.c", tmp_path / "sz"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "nmpc_amd.h"\nint main(void){printf("%zu %zu %zu %zu\\n", sizeof(nmpc_scan_args), '
+                   'offsetof(nmpc_scan_args, A), offsetof(nmpc_scan_args, dlast), offsetof(nmpc_scan_args, workspace_bytes));return 0;}\n')
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
+    S = _lib.ScanArgs
+    assert list(map(int, subprocess.check_output([str(exe)]).split())) == [ctypes.sizeof(S), S.A.offset, S.dlast.offset, S.workspace_bytes.offset]
+    L = _lib.lib()
+    buf = (ctypes.c_float * 64)()
+    p = ctypes.addressof(buf)
+    def args(**kw):
+        s = S()
+        s.struct_size, s.nb, s.L, s.D, s.N, s.G = ctypes.sizeof(S), 1, 4, 4, 4, 1
+        for k in ("u", "dt", "B", "C", "A", "y", "last", "saved", "dy", "du", "ddt", "dB", "dC", "dA"):
+            setattr(s, k, p)
+        for k, v in kw.items():
+            setattr(s, k, v)
+        return ctypes.addressof(s), s
+    for kw in (dict(struct_size=8), dict(dtype=7), dict(nb=-1), dict(L=-1), dict(D=0), dict(N=0), dict(N=65), dict(G=3), dict(G=0), dict(A=None),
+               dict(u=None), dict(C=None), dict(y=None), dict(nb=1 << 20, D=1 << 12)):
+        at, hold = args(**kw)
+        assert L.nmpc_lpv_scan(at, None) != 0 and L.nmpc_last_error(), kw
+    for kw in (dict(saved=None), dict(dy=None), dict(dA=None), dict(dB=None), dict(z=p), dict(D_skip=p), dict(dt_bias=p), dict(workspace=None),
+               dict(workspace=p, workspace_bytes=16)):
+        at, hold = args(**kw)
+        assert L.nmpc_lpv_scan_bwd(at, None) != 0 and L.nmpc_last_error(), kw
+    for kw in (dict(last=None), dict(u=None), dict(y=None)):
+        at, hold = args(**kw)
+        assert L.nmpc_lpv_scan_step(at, None) != 0, kw
+    assert L.nmpc_lpv_scan(None, None) != 0
+    at, hold = args(nb=0)
+    assert L.nmpc_lpv_scan(at, None) == 0 and L.nmpc_lpv_scan_step(at, None) == 0
+    assert L.nmpc_lpv_scan_saved_bytes(2, 33, 8, 5) == 2 * 2 * 8 * 8 * 4

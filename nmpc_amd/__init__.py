@@ -11,4 +11,4 @@ from .target import GetABC, getXsUs_Cs, getXsUs  # noqa: F401
 from .lpvrk4 import lpv_rk4  # noqa: F401
 from .reference import stackReferences, randomLevelReference, random_level_batch, lpv_histogram, comp_time_stats  # noqa: F401
 from .seq import (causal_conv, causal_conv_fwd, causal_conv_bwd, causal_conv_step, lpv_scan, lpv_scan_fwd,  # noqa: F401
-                  lpv_scan_bwd, lpv_scan_step)
+                  lpv_scan_bwd, lpv_scan_step, gated_ffn, gated_ffn_fwd, gated_ffn_bwd)

@@ -356,3 +356,77 @@ def lpv_scan_step(state, u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=
     s.y, s.last = y.data_ptr(), state.data_ptr()
     _call(u.device, what, lib().nmpc_lpv_scan_step, ctypes.addressof(s))
     return y
+
+
+# ---- gated feed-forward projections ---------------------------------------------------------------------------------
+def _ffn_args(what, x, w_gate, w_up, act):
+    _need(torch.is_tensor(x) and x.dim() >= 1, what, "x must be [..., inputs]")
+    _need(x.dtype in _DTYPES, what, "x is %s, expected float32, bfloat16 or float16", x.dtype)
+    k = x.shape[-1]
+    _need(torch.is_tensor(w_gate) and w_gate.dim() == 2 and w_gate.shape[1] == k and k >= 1 and w_gate.shape[0] >= 1, what,
+          "w_gate must be [hidden, %d]", k)
+    _need(act in ("silu", "gelu", "tanh", "sigmoid"), what, "activation %r (silu, gelu, tanh or sigmoid)", act)
+    w_gate = _samples(what, "w_gate", w_gate, w_gate.shape, x.dtype)
+    w_up = _samples(what, "w_up", w_up, w_gate.shape, x.dtype)
+    if w_gate.stride(0) != w_up.stride(0):
+        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    rows = x.reshape(-1, k)
+    return rows if rows.stride(-1) == 1 or k == 1 else rows.contiguous(), w_gate, w_up
+
+
+def _ffn_work(x, w, backward):
+    size = lib().nmpc_gated_ffn_workspace_bytes(_DTYPES[x.dtype], x.shape[0], x.shape[1], w.shape[0], backward)
+    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
+
+
+def _ffn_fwd(what, x, w_gate, w_up, act, want_saved):
+    rows, w_gate, w_up = _ffn_args(what, x, w_gate, w_up, act)
+    _on_gpu(what, rows, w_gate, w_up)
+    (m, k), f = rows.shape, w_gate.shape[0]
+    h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
+    pre = torch.empty((2, m, f), dtype=torch.float32, device=x.device) if want_saved else None
+    work, size = _ffn_work(rows, w_gate, 0)
+    _call(x.device, what, lib().nmpc_gated_ffn, _DTYPES[x.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate), w_gate.stride(0),
+          _p(w_up), w_up.stride(0), _ACTS[act], _p(h), _p(pre), _p(work), size)
+    return h, (rows, w_gate, w_up, pre)
+
+
+def gated_ffn_fwd(x, w_gate, w_up, act="silu"):
+    """gated_ffn that keeps what its gradient needs: (h, saved).  Besides the inputs that is both projections in fp32."""
+    with torch.no_grad():
+        h, tensors = _ffn_fwd("gated_ffn_fwd", x, w_gate, w_up, act, True)
+    return h, Saved("gated_ffn", tensors, (act, tuple(x.shape)))
+
+
+def gated_ffn_bwd(saved, dh):
+    """Gradients (dx, dw_gate, dw_up) of gated_ffn_fwd's call, in the inputs' type; dh like h."""
+    what = "gated_ffn_bwd"
+    (rows, w_gate, w_up, pre), (act, shape) = _saved("gated_ffn", saved)
+    (m, k), f = rows.shape, w_gate.shape[0]
+    dh = _samples(what, "dh", dh, shape[:-1] + (f,), rows.dtype).reshape(m, f)
+    _on_gpu(what, rows, dh)
+    dx = torch.empty(shape, dtype=rows.dtype, device=rows.device)
+    dwg, dwu = (torch.empty((f, k), dtype=rows.dtype, device=rows.device) for _ in range(2))
+    work, size = _ffn_work(rows, w_gate, 1)
+    _call(rows.device, what, lib().nmpc_gated_ffn_bwd, _DTYPES[rows.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate),
+          w_gate.stride(0), _p(w_up), w_up.stride(0), _ACTS[act], _p(pre), _p(dh), dh.stride(0), _p(dx), _p(dwg), _p(dwu), _p(work), size)
+    return dx, dwg, dwu
+
+
+def gated_ffn(x, w_gate, w_up, act="silu"):
+    """h = act(x w_gate') * (x w_up'): both projections, the activation and the product in one kernel.
+
+    x [..., inputs]; w_gate, w_up [hidden, inputs] of x's type; act "silu", "gelu" (erf), "tanh" or "sigmoid".  One row or a
+    few (tokens of running sequences) and many rows (prompts, training) take kernels of their own."""
+    what = "gated_ffn"
+    if not _records(what, x, w_gate, w_up):
+        with torch.no_grad():
+            return _ffn_fwd(what, x, w_gate, w_up, act, False)[0]
+
+    def fwd():
+        h, saved = gated_ffn_fwd(x, w_gate, w_up, act)
+        return (h,), saved
+
+    def bwd(saved, dh):
+        return (None, None, None) if dh is None else gated_ffn_bwd(saved, dh)
+    return _Recorded.apply(fwd, bwd, x, w_gate, w_up)[0]

@@ -142,3 +142,40 @@ def test_scan_abi(tmp_path):
     at, hold = args(nb=0)
     assert L.nmpc_lpv_scan(at, None) == 0 and L.nmpc_lpv_scan_step(at, None) == 0
     assert L.nmpc_lpv_scan_saved_bytes(2, 33, 8, 5) == 2 * 2 * 8 * 8 * 4
+
+
+def test_oracle_ffn_gradient_against_differences():
+    g = rng(3)
+    for name in ("silu", "gelu", "tanh", "sigmoid"):
+        assert torch.autograd.gradcheck(lambda *a: oracle.gated_ffn(*a, name), (_double(g, 3, 4), _double(g, 5, 4), _double(g, 5, 4)))
+
+
+def test_ffn_refusals():
+    x, w = torch.zeros(3, 8), torch.zeros(6, 8)
+    bad = [(dict(x=x.double()), "float32, bfloat16"), (dict(w_gate=torch.zeros(6, 7)), r"\[hidden, 8\]"), (dict(w_up=torch.zeros(5, 8)), "w_up must be"),
+           (dict(w_up=w.half()), "the samples are"), (dict(w_gate=torch.zeros(8)), "w_gate must be"), (dict(act="relu"), "activation"),
+           (dict(act=None), "activation"), (dict(w_gate=torch.zeros(0, 8), w_up=torch.zeros(0, 8)), "w_gate must be")]
+    for change, text in bad:
+        for fn in (nmpc_amd.gated_ffn, nmpc_amd.gated_ffn_fwd):
+            with pytest.raises(nmpc_amd.NmpcError, match=text):
+                fn(**{**dict(x=x, w_gate=w, w_up=w), **change})
+    with pytest.raises(nmpc_amd.NmpcError, match="gated_ffn_fwd returned"):
+        nmpc_amd.gated_ffn_bwd(None, x)
+
+
+def test_ffn_abi_refusals():
+    L = _lib.lib()
+    buf = (ctypes.c_float * 64)()
+    p = ctypes.addressof(buf)
+    def fwd(dtype=0, m=4, k=4, f=4, x=p, wg=p, wu=p, ldu=4, act=1, h=p):
+        return L.nmpc_gated_ffn(dtype, m, k, f, x, 4, wg, 4, wu, ldu, act, h, None, None, 0, None)
+    for kw in (dict(dtype=-1), dict(m=-1), dict(k=0), dict(f=0), dict(x=None), dict(wg=None), dict(wu=None), dict(h=None), dict(act=0), dict(act=5),
+               dict(ldu=8), dict(m=1 << 22)):
+        assert fwd(**kw) != 0 and L.nmpc_last_error(), kw
+    assert fwd(m=0, x=None, h=None) == 0
+    need = L.nmpc_gated_ffn_workspace_bytes(1, 100, 64, 128, 1)
+    assert need > 0
+    rc = L.nmpc_gated_ffn_bwd(1, 100, 64, 128, p, 64, p, 64, p, 64, 1, p, p, 128, p, p, p, p, need - 1, None)
+    assert rc != 0 and b"workspace" in L.nmpc_last_error()
+    rc = L.nmpc_gated_ffn_bwd(1, 100, 64, 128, p, 64, p, 64, p, 64, 1, None, p, 128, p, p, p, p, need, None)
+    assert rc != 0 and b"null" in L.nmpc_last_error()

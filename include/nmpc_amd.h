@@ -334,9 +334,10 @@ int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream);
 /* Gated feed-forward projections: h = act(x Wg') o (x Wu'), act = SiLU, GELU (erf), tanh or sigmoid; x[M,K], Wg / Wu[F,K],
  * h[M,F], all of one element type; row strides x_ld, wg_ld = wu_ld, dh_ld in elements, rows contiguous, outputs contiguous.
  * pre (NULL = no gradient wanted): fp32 [2][M][F], both projections before the activation, for _bwd.
- * _bwd: dh -> dx[M,K], dwg / dwu[F,K].  workspace: nmpc_gated_ffn_workspace_bytes (0 for some sizes), contents need not be
- * preserved; calls that overlap in time need one each. */
-unsigned long long nmpc_gated_ffn_workspace_bytes(int dtype, int M, int K, int F, int backward);
+ * _bwd: dh -> dx[M,K], dwg / dwu[F,K].  workspace: nmpc_gated_ffn_workspace_bytes (0 for some sizes; copy = 1 unless x and the
+ * weights start on 16 bytes and have row strides of whole 16 bytes), contents need not be preserved; calls that overlap in
+ * time need one each. */
+unsigned long long nmpc_gated_ffn_workspace_bytes(int dtype, int M, int K, int F, int backward, int copy);
 int nmpc_gated_ffn(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld, const void* wu,
                    long long wu_ld, int act, void* h, float* pre, void* workspace, unsigned long long workspace_bytes, void* stream);
 int nmpc_gated_ffn_bwd(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld, const void* wu,

@@ -374,8 +374,9 @@ def _ffn_args(what, x, w_gate, w_up, act):
     return rows if rows.stride(-1) == 1 or k == 1 else rows.contiguous(), w_gate, w_up
 
 
-def _ffn_work(x, w, backward):
-    size = lib().nmpc_gated_ffn_workspace_bytes(_DTYPES[x.dtype], x.shape[0], x.shape[1], w.shape[0], backward)
+def _ffn_work(x, w_gate, w_up, backward):
+    bits = w_gate.data_ptr() | w_up.data_ptr() | x.data_ptr() | (x.stride(0) | w_gate.stride(0)) * x.element_size()
+    size = lib().nmpc_gated_ffn_workspace_bytes(_DTYPES[x.dtype], x.shape[0], x.shape[1], w_gate.shape[0], backward, bits % 16 != 0)
     return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
 
 
@@ -385,7 +386,7 @@ def _ffn_fwd(what, x, w_gate, w_up, act, want_saved):
     (m, k), f = rows.shape, w_gate.shape[0]
     h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
     pre = torch.empty((2, m, f), dtype=torch.float32, device=x.device) if want_saved else None
-    work, size = _ffn_work(rows, w_gate, 0)
+    work, size = _ffn_work(rows, w_gate, w_up, 0)
     _call(x.device, what, lib().nmpc_gated_ffn, _DTYPES[x.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate), w_gate.stride(0),
           _p(w_up), w_up.stride(0), _ACTS[act], _p(h), _p(pre), _p(work), size)
     return h, (rows, w_gate, w_up, pre)
@@ -407,7 +408,7 @@ def gated_ffn_bwd(saved, dh):
     _on_gpu(what, rows, dh)
     dx = torch.empty(shape, dtype=rows.dtype, device=rows.device)
     dwg, dwu = (torch.empty((f, k), dtype=rows.dtype, device=rows.device) for _ in range(2))
-    work, size = _ffn_work(rows, w_gate, 1)
+    work, size = _ffn_work(rows, w_gate, w_up, 1)
     _call(rows.device, what, lib().nmpc_gated_ffn_bwd, _DTYPES[rows.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate),
           w_gate.stride(0), _p(w_up), w_up.stride(0), _ACTS[act], _p(pre), _p(dh), dh.stride(0), _p(dx), _p(dwg), _p(dwu), _p(work), size)
     return dx, dwg, dwu

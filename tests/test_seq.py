@@ -173,7 +173,7 @@ def test_ffn_abi_refusals():
                dict(ldu=8), dict(m=1 << 22)):
         assert fwd(**kw) != 0 and L.nmpc_last_error(), kw
     assert fwd(m=0, x=None, h=None) == 0
-    need = L.nmpc_gated_ffn_workspace_bytes(1, 100, 64, 128, 1)
+    need = L.nmpc_gated_ffn_workspace_bytes(1, 100, 64, 128, 1, 0)
     assert need > 0
     rc = L.nmpc_gated_ffn_bwd(1, 100, 64, 128, p, 64, p, 64, p, 64, 1, p, p, 128, p, p, p, p, need - 1, None)
     assert rc != 0 and b"workspace" in L.nmpc_last_error()

@@ -12,12 +12,14 @@
 // P lanes of a channel do not repeat them; B and C are read from LDS as one 16-byte access per lane.
 // What bounds it: VALU issue.  A state and step costs 2 (exp2) + 4 slots forward; the bytes are 8 a channel and step in bf16.
 #include <algorithm>
+#include <type_traits>
 
 #include "seq_common.h"
 
 namespace nmpc {
 
 constexpr int SCAN_T = 32;             // steps of a tile
+constexpr int SCAN_SAVE = 16;          // the forward pass saves the state before every 16th step: a tile of the backward pass
 constexpr int SCAN_THREADS = 256;
 
 struct ScanDev {
@@ -28,24 +30,51 @@ struct ScanDev {
     float *pA, *pDb, *pBC;             // partial sums (backward)
 };
 
+// softplus(x) = max(x, 0) + log(1 + e) with e = e^-|x| <= 1, and log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3: a polynomial in s^2
+// through the Chebyshev points of [0, 1/9] (off by 8e-9 of the value), so that small values keep their relative accuracy
 __device__ __forceinline__ float softplus(float x) {
-    if (x > 20.f) return x;            // e^-20 is below half a step of x
-    return log1pf(__builtin_amdgcn_exp2f(x * LOG2E));
+    const float e = __builtin_amdgcn_exp2f(-LOG2E * fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    const float r = 1.f + q * (0.33333161f + q * (0.20012298f + q * (0.13982579f + q * 0.1407889f)));
+    return fmaxf(x, 0.f) + 2.f * s * r;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-    const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
-    return v + __builtin_bit_cast(float, o);
+template <int CTRL, int BANKS = 0xf>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, BANKS, true));
 }
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_SHL4 = 0x104, DPP_ROR8 = 0x128, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
+
 // sum over the P lanes of a channel; every lane gets the same bits
 template <int P>
 __device__ __forceinline__ float sum_lanes(float v) {
-    if constexpr (P >= 2) v = dpp_add<0xB1>(v);       // quad_perm [1,0,3,2]
-    if constexpr (P >= 4) v = dpp_add<0x4E>(v);       // quad_perm [2,3,0,1]
-    if constexpr (P >= 8) v = dpp_add<0x141>(v);      // mirror within 8
-    if constexpr (P >= 16) v = dpp_add<0x140>(v);     // mirror within 16
+    if constexpr (P >= 2) v += dpp<DPP_XOR1>(v);
+    if constexpr (P >= 4) v += dpp<DPP_XOR2>(v);
+    if constexpr (P >= 8) v += dpp<DPP_HALF_MIRROR>(v);
+    if constexpr (P >= 16) v += dpp<DPP_MIRROR>(v);
     return v;
+}
+
+// The same for the values of S = min(P, 4) steps at once: lane q < S gets the sum of step q (others: nothing of use).  A lane of a pair
+// keeps one of two values and hands the other over, so that each stage halves the values instead of repeating the sum.
+template <int P>
+struct Steps {
+    static constexpr int S = P < 4 ? P : 4;
+};
+template <int P>
+__device__ __forceinline__ float sum_steps(const float (&y)[Steps<P>::S], int lane) {
+    if constexpr (P == 1) return y[0];
+    else {
+        const bool odd = lane & 1;
+        float r = (odd ? y[1] : y[0]) + dpp<DPP_XOR1>(odd ? y[0] : y[1]);
+        if constexpr (P >= 4) {
+            const bool high = lane & 2;
+            const float t = (odd ? y[3] : y[2]) + dpp<DPP_XOR1>(odd ? y[2] : y[3]);
+            r = (high ? t : r) + dpp<DPP_XOR2>(high ? r : t);
+        }
+        if constexpr (P >= 16) r += dpp<DPP_ROR8>(r);
+        if constexpr (P >= 8) r += dpp<DPP_SHL4>(r);      // lane i += lane i + 4 (within 16; the lanes that count have a partner)
+        return r;
+    }
 }
 
 // Where a workgroup works: channel block of a group, chunk, sequence.
@@ -65,15 +94,82 @@ struct ScanPlace {
     }
 };
 
-// rows t0 .. t0+31 of B or C (of this group) as fp32, zero past the sequence and past N
-template <typename T, int P>
-__device__ __forceinline__ void stage_bc(float (*dst)[4 * P], const void* src, long long bs, long long ts, int b, int g, int N, int t0, int len) {
-    const T* p = (const T*)src + b * bs + (long long)g * N;
-    for (int e = threadIdx.x; e < SCAN_T * 4 * P; e += SCAN_THREADS) {
-        const int t = e / (4 * P), n = e % (4 * P);
-        dst[t][n] = (t0 + t < len && n < N) ? (float)p[(long long)(t0 + t) * ts + n] : 0.f;
+// A thread's part of a tile of R steps: V neighbouring channels (column `cc`) of PER rows.  V = 2: one access covers a pair, so that a
+// row of 64 channels is read by 32 lanes and its staged values are written to LDS without bank conflicts.
+template <int P, int V, int R>
+struct Part {
+    static constexpr int CH = SCAN_THREADS / P, COLS = CH / V, STEP = SCAN_THREADS / COLS, PER = R / STEP;
+    static_assert(R % STEP == 0, "whole rows");
+    int cc, t;
+    __device__ __forceinline__ Part() : cc((threadIdx.x % COLS) * V), t(threadIdx.x / COLS) {}
+    __device__ __forceinline__ int row(int i) const { return t + i * STEP; }
+};
+
+// One sample tensor as a thread sees it: uniform row addresses plus a 32-bit offset of its own (the host checks that it fits).
+template <typename T, int V, typename PART>
+struct Stream {
+    const T* p;
+    long long ts;
+    unsigned off;
+    __device__ __forceinline__ Stream(const void* base, long long bs, long long ts_, int b, int c0, const PART& part)
+        : p(base ? (const T*)base + b * bs + c0 : nullptr), ts(ts_), off((unsigned)((part.t * (int)ts_ + part.cc) * (int)sizeof(T))) {}
+    template <bool WHOLE>
+    __device__ __forceinline__ void fetch(Vec<T, V> (&v)[PART::PER], const PART& part, int t0, int end, bool ok) const {
+#pragma unroll
+        for (int i = 0; i < PART::PER; ++i)
+            if (WHOLE || (ok && t0 + part.row(i) < end))
+                v[i] = *reinterpret_cast<const Vec<T, V>*>((const char*)(p + (long long)(t0 + i * PART::STEP) * ts) + off);
+    }
+};
+
+// f(true) for a tile whose steps and channels all count, f(false) otherwise
+template <typename F>
+__device__ __forceinline__ void whole_or_not(bool whole, F f) {
+    if (whole) f(std::integral_constant<bool, true>{});
+    else f(std::integral_constant<bool, false>{});
+}
+
+// delta of a thread's samples
+template <typename T, int V, int PER>
+__device__ __forceinline__ void deltas(float (&d)[PER][V], const Vec<T, V> (&raw)[PER], const float (&bias)[V], int with_softplus) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = (float)raw[i].v[j] + bias[j];
+    if (with_softplus) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[i][j] = softplus(d[i][j]);
     }
 }
+template <int V>
+__device__ __forceinline__ void put_pairs(float2* dst, const float (&a)[V], const float (&b)[V]) {
+    if constexpr (V == 2) *reinterpret_cast<float4*>(dst) = make_float4(a[0], b[0], a[1], b[1]);
+    else *dst = make_float2(a[0], b[0]);
+}
+
+// rows of B or C (of this group) as fp32 into LDS, zero past the sequence and past N
+template <typename T, int P, int R>
+struct Shared {
+    static constexpr int PER = (R * 4 * P + SCAN_THREADS - 1) / SCAN_THREADS;
+    T v[PER];
+    __device__ __forceinline__ void fetch(const T* p, long long ts, int N, int t0, int len) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = threadIdx.x + i * SCAN_THREADS, t = t0 + e / (4 * P), n = e % (4 * P);
+            v[i] = (T)0.f;
+            if (e < R * 4 * P && t < len && n < N) v[i] = p[(long long)t * ts + n];
+        }
+    }
+    __device__ __forceinline__ void put(float (*dst)[4 * P]) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = threadIdx.x + i * SCAN_THREADS;
+            if (e < R * 4 * P) (&dst[0][0])[e] = (float)v[i];
+        }
+    }
+};
 
 template <int P>
 __device__ __forceinline__ void load_A(const ScanDev& s, int c, bool ok, int q, float (&a)[4]) {
@@ -94,85 +190,152 @@ __device__ __forceinline__ void store_states(float* p, int N, int q, const float
     for (int i = 0; i < 4; ++i)
         if (4 * q + i < N) p[4 * q + i] = x[i];
 }
+// the same in the library's own arrays [..][4P]
+__device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void store_four(float* p, const float (&x)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// LDS operands of S steps
+template <int P, bool SUMMARY>
+struct Group {
+    static constexpr int S = Steps<P>::S;
+    float2 dx[S];
+    float b[S][4], c[SUMMARY ? 1 : S][4];
+    template <typename DX, typename B, typename C>
+    __device__ __forceinline__ void read(const DX& sDX, const B& sB, const C& sC, int t, int ch, int q) {
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            dx[k] = sDX[t + k][ch];
+            load_four(&sB[t + k][4 * q], b[k]);
+            if constexpr (!SUMMARY) load_four(&sC[t + k][4 * q], c[k]);
+        }
+    }
+};
 
 // SUMMARY: only what the steps of a chunk do to a state: x_end = exp2(a dsum) x_begin + xin, started from zero.
 // Otherwise the scan itself from the state before the chunk.
-template <typename T, int P, bool SUMMARY>
-__global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanDev s) {
-    constexpr int CH = SCAN_THREADS / P;
-    __shared__ float2 sDX[SCAN_T][CH];                // delta, delta u
-    __shared__ float sB[SCAN_T][4 * P], sC[SUMMARY ? 1 : SCAN_T][4 * P], sY[SUMMARY ? 1 : SCAN_T][CH];
+template <typename T, int P, int V, bool SUMMARY>
+__global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : P == 2 ? 2 : 3) void scan_fwd_kernel(ScanDev s) {
+    constexpr int CH = SCAN_THREADS / P, S = Steps<P>::S;
+    __shared__ __attribute__((aligned(16))) float2 sDX[SCAN_T][CH];   // delta, delta u
+    __shared__ __attribute__((aligned(16))) float sB[SCAN_T][4 * P], sC[SUMMARY ? 1 : SCAN_T][4 * P], sY[SUMMARY ? 1 : SCAN_T][CH];
     const nmpc_scan_args& a = s.a;
     const ScanPlace<P> at(s);
+    const Part<P, V, SCAN_T> part;
+    constexpr int PER = Part<P, V, SCAN_T>::PER;
     const int tid = threadIdx.x, c = tid / P, q = tid % P, ch = at.c0 + c;
-    const bool ok = c < at.nvalid;
+    const bool ok = c < at.nvalid, mine = part.cc < at.nvalid;
     float A[4], x[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
     load_A<P>(s, ch, ok, q, A);
-    const long long part = ((long long)(at.b * s.nch + at.chunk) * a.D + ch) * (4 * P) + 4 * q;
+    float* chunk_state = s.xin + ((long long)(at.b * s.nch + at.chunk) * a.D + ch) * (4 * P) + 4 * q;
     if (!SUMMARY && ok) {
-        if (s.nch > 1) load_states(s.xin + part - 4 * q, 4 * P, q, x);
+        if (s.nch > 1) load_four(chunk_state, x);
         else if (a.start) load_states(a.start + ((long long)at.b * a.D + ch) * a.N, a.N, q, x);
     }
-    const T* u = (const T*)a.u + at.b * a.u_bs + at.c0;
-    const T* dt = (const T*)a.dt + at.b * a.dt_bs + at.c0;
-    const T* z = a.z ? (const T*)a.z + at.b * a.z_bs + at.c0 : nullptr;
+    using PT = Part<P, V, SCAN_T>;
+    const Stream<T, V, PT> u(a.u, a.u_bs, a.u_ts, at.b, at.c0, part), dt(a.dt, a.dt_bs, a.dt_ts, at.b, at.c0, part),
+        z(SUMMARY ? nullptr : a.z, a.z_bs, a.z_ts, at.b, at.c0, part);
+    const T* B = (const T*)a.B + at.b * a.B_bs + (long long)at.g * a.N;
+    const T* C = (const T*)a.C + at.b * a.C_bs + (long long)at.g * a.N;
+    float bias[V], skip[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = a.dt_bias && mine ? a.dt_bias[at.c0 + part.cc + j] : 0.f;
+        skip[j] = !SUMMARY && a.D_skip && mine ? a.D_skip[at.c0 + part.cc + j] : 0.f;
+    }
     const int tile0 = at.chunk * s.tpc, tile1 = min(tile0 + s.tpc, s.ntile);
+    auto whole = [&](int t0) { return at.nvalid == CH && t0 + SCAN_T <= at.len; };
+    Vec<T, V> nd[PER], nu[PER], nz[PER], cu[PER], cz[PER];           // the next tile's samples, this one's
+    Shared<T, P, SCAN_T> nB, nC;
+    auto next = [&](int t0) {
+        whole_or_not(whole(t0), [&](auto w) {
+            dt.template fetch<w.value>(nd, part, t0, at.len, mine);
+            u.template fetch<w.value>(nu, part, t0, at.len, mine);
+            if (!SUMMARY && z.p) z.template fetch<w.value>(nz, part, t0, at.len, mine);
+        });
+        nB.fetch(B, a.B_ts, a.N, t0, at.len);
+        if constexpr (!SUMMARY) nC.fetch(C, a.C_ts, a.N, t0, at.len);
+    };
+    if (tile0 < tile1) next(tile0 * SCAN_T);
     for (int tile = tile0; tile < tile1; ++tile) {
         const int t0 = tile * SCAN_T;
-        __syncthreads();
-        for (int e = tid; e < SCAN_T * CH; e += SCAN_THREADS) {
-            const int t = e / CH, cc = e % CH;
-            float d = 0.f, du = 0.f;
-            if (t0 + t < at.len && cc < at.nvalid) {
-                d = (float)dt[(long long)(t0 + t) * a.dt_ts + cc] + (a.dt_bias ? a.dt_bias[at.c0 + cc] : 0.f);
-                if (a.softplus) d = softplus(d);
-                du = d * (float)u[(long long)(t0 + t) * a.u_ts + cc];
-            }
-            sDX[t][cc] = make_float2(d, du);
-        }
-        stage_bc<T, P>(sB, a.B, a.B_bs, a.B_ts, at.b, at.g, a.N, t0, at.len);
-        if constexpr (!SUMMARY) {
-            stage_bc<T, P>(sC, a.C, a.C_bs, a.C_ts, at.b, at.g, a.N, t0, at.len);
-            if (a.saved && ok) store_states((float*)a.saved + (((long long)at.b * s.ntile + tile) * a.D + ch) * (4 * P), 4 * P, q, x);
-        }
-        __syncthreads();
-#pragma unroll 4
-        for (int t = 0; t < SCAN_T; ++t) {
-            const float2 dx = sDX[t][c];
-            const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][4 * q]);
-            const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+        whole_or_not(whole(t0), [&](auto w) {
+            float d[PER][V];
+            deltas(d, nd, bias, a.softplus);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_exp2f(dx.x * A[i]) * x[i] + dx.y * b[i];
-            if constexpr (SUMMARY) {
-                total += dx.x;
-            } else {
-                const float4 c4 = *reinterpret_cast<const float4*>(&sC[t][4 * q]);
-                const float y = sum_lanes<P>(c4.x * x[0] + c4.y * x[1] + c4.z * x[2] + c4.w * x[3]);
-                if (q == 0) sY[t][c] = y;
-            }
-        }
-        if constexpr (!SUMMARY) {
-            __syncthreads();
-            T* y = (T*)a.y + ((long long)at.b * a.L + t0) * a.D + at.c0;
-            for (int e = tid; e < SCAN_T * CH; e += SCAN_THREADS) {
-                const int t = e / CH, cc = e % CH;
-                if (t0 + t >= a.L || cc >= at.nvalid) continue;
-                float v = 0.f;
-                if (t0 + t < at.len) {
-                    v = sY[t][cc];
-                    if (a.D_skip) v += a.D_skip[at.c0 + cc] * (float)u[(long long)(t0 + t) * a.u_ts + cc];
-                    if (z) {
-                        const float zz = (float)z[(long long)(t0 + t) * a.z_ts + cc];
-                        v *= zz * sigmoid(zz);
-                    }
+            for (int i = 0; i < PER; ++i) {
+                float du[V];
+                const bool in = w.value || (mine && t0 + part.row(i) < at.len);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    du[j] = in ? d[i][j] * (float)nu[i].v[j] : 0.f;
+                    d[i][j] = in ? d[i][j] : 0.f;
                 }
-                y[(long long)t * a.D + cc] = (T)v;
+                put_pairs<V>(&sDX[part.row(i)][part.cc], d[i], du);
+                cu[i] = nu[i];
+                cz[i] = nz[i];
             }
+        });
+        nB.put(sB);
+        if constexpr (!SUMMARY) nC.put(sC);
+        __syncthreads();
+        if (tile + 1 < tile1) next(t0 + SCAN_T);
+        // groups of S steps; the next group's operands are read from LDS while this one is computed
+        Group<P, SUMMARY> cur, ahead;
+        cur.read(sDX, sB, sC, 0, c, q);
+#pragma unroll
+        for (int t4 = 0; t4 < SCAN_T; t4 += S) {
+            if (t4 + S < SCAN_T) ahead.read(sDX, sB, sC, t4 + S, c, q);
+            if constexpr (!SUMMARY) {
+                if (t4 % SCAN_SAVE == 0 && a.saved && ok && t0 + t4 < a.L)
+                    store_four((float*)a.saved + (((long long)at.b * ((a.L + SCAN_SAVE - 1) / SCAN_SAVE) + (t0 + t4) / SCAN_SAVE) * a.D + ch) * (4 * P) + 4 * q, x);
+            }
+            float y[S];
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+                const float2 dx = cur.dx[k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_exp2f(dx.x * A[i]) * x[i] + dx.y * cur.b[k][i];
+                if constexpr (SUMMARY) total += dx.x;
+                else y[k] = cur.c[k][0] * x[0] + cur.c[k][1] * x[1] + cur.c[k][2] * x[2] + cur.c[k][3] * x[3];
+            }
+            if constexpr (!SUMMARY) {
+                const float r = sum_steps<P>(y, tid);
+                if (P <= 4 || q < 4) sY[t4 + (q & 3)][c] = r;
+            }
+            cur = ahead;
+        }
+        __syncthreads();
+        if constexpr (!SUMMARY) {
+            T* y = (T*)a.y + ((long long)at.b * a.L + t0) * a.D + at.c0;
+            whole_or_not(whole(t0), [&](auto w) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int t = part.row(i);
+                    if (!w.value && (!mine || t0 + t >= a.L)) continue;
+                    const bool in = w.value || t0 + t < at.len;
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        float v = sY[t][part.cc + j] + skip[j] * (float)cu[i].v[j];
+                        if (z.p) {
+                            const float zz = (float)cz[i].v[j];
+                            v *= zz * sigmoid(zz);
+                        }
+                        o.v[j] = (T)(in ? v : 0.f);
+                    }
+                    store_vec(y + (long long)(i * PT::STEP) * a.D + (unsigned)(part.t * a.D + part.cc), o);
+                }
+            });
         }
     }
     if (!ok) return;
     if constexpr (SUMMARY) {
-        store_states(s.xin + part - 4 * q, 4 * P, q, x);
+        store_four(chunk_state, x);
         if (q == 0) s.dsum[(long long)(at.b * s.nch + at.chunk) * a.D + ch] = total;
     } else if (a.last && at.chunk == s.nch - 1) {
         store_states(a.last + ((long long)at.b * a.D + ch) * a.N, a.N, q, x);
@@ -201,201 +364,306 @@ __global__ __launch_bounds__(256) void scan_chunks_kernel(ScanDev s, int NP) {
 }
 
 // The adjoint's summary of a chunk: lam before its first step, times that step's decay, started from zero behind its last.
-template <typename T, int P>
+template <typename T, int P, int V>
 __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_summary_kernel(ScanDev s) {
     constexpr int CH = SCAN_THREADS / P;
-    __shared__ float2 sDG[SCAN_T][CH];                // delta, g
-    __shared__ float sC[SCAN_T][4 * P];
+    __shared__ __attribute__((aligned(16))) float2 sDG[SCAN_T][CH];   // delta, g
+    __shared__ __attribute__((aligned(16))) float sC[SCAN_T][4 * P];
     const nmpc_scan_args& a = s.a;
     const ScanPlace<P> at(s);
+    const Part<P, V, SCAN_T> part;
+    constexpr int PER = Part<P, V, SCAN_T>::PER;
     const int tid = threadIdx.x, c = tid / P, q = tid % P, ch = at.c0 + c;
-    const bool ok = c < at.nvalid;
-    float A[4], lam[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
+    const bool ok = c < at.nvalid, mine = part.cc < at.nvalid;
+    float A[4], lam[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f, bias[V];
     load_A<P>(s, ch, ok, q, A);
-    const T* dt = (const T*)a.dt + at.b * a.dt_bs + at.c0;
-    const T* z = a.z ? (const T*)a.z + at.b * a.z_bs + at.c0 : nullptr;
-    const T* dy = (const T*)a.dy + at.b * a.dy_bs + at.c0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) bias[j] = a.dt_bias && mine ? a.dt_bias[at.c0 + part.cc + j] : 0.f;
+    using PT = Part<P, V, SCAN_T>;
+    const Stream<T, V, PT> dt(a.dt, a.dt_bs, a.dt_ts, at.b, at.c0, part), z(a.z, a.z_bs, a.z_ts, at.b, at.c0, part),
+        dy(a.dy, a.dy_bs, a.dy_ts, at.b, at.c0, part);
+    const T* C = (const T*)a.C + at.b * a.C_bs + (long long)at.g * a.N;
     const int tile0 = at.chunk * s.tpc, tile1 = min(tile0 + s.tpc, s.ntile);
+    auto whole = [&](int t0) { return at.nvalid == CH && t0 + SCAN_T <= at.len; };
+    Vec<T, V> nd[PER], ng[PER], nz[PER];
+    Shared<T, P, SCAN_T> nC;
+    auto next = [&](int t0) {
+        whole_or_not(whole(t0), [&](auto w) {
+            dt.template fetch<w.value>(nd, part, t0, at.len, mine);
+            dy.template fetch<w.value>(ng, part, t0, at.len, mine);
+            if (z.p) z.template fetch<w.value>(nz, part, t0, at.len, mine);
+        });
+        nC.fetch(C, a.C_ts, a.N, t0, at.len);
+    };
+    if (tile0 < tile1) next((tile1 - 1) * SCAN_T);
     for (int tile = tile1 - 1; tile >= tile0; --tile) {
         const int t0 = tile * SCAN_T;
-        __syncthreads();
-        for (int e = tid; e < SCAN_T * CH; e += SCAN_THREADS) {
-            const int t = e / CH, cc = e % CH;
-            float d = 0.f, g = 0.f;
-            if (t0 + t < at.len && cc < at.nvalid) {
-                d = (float)dt[(long long)(t0 + t) * a.dt_ts + cc] + (a.dt_bias ? a.dt_bias[at.c0 + cc] : 0.f);
-                if (a.softplus) d = softplus(d);
-                g = (float)dy[(long long)(t0 + t) * a.dy_ts + cc];
-                if (z) {
-                    const float zz = (float)z[(long long)(t0 + t) * a.z_ts + cc];
-                    g *= zz * sigmoid(zz);
+        whole_or_not(whole(t0), [&](auto w) {
+            float d[PER][V];
+            deltas(d, nd, bias, a.softplus);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                float g[V];
+                const bool in = w.value || (mine && t0 + part.row(i) < at.len);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    g[j] = (float)ng[i].v[j];
+                    if (z.p) {
+                        const float zz = (float)nz[i].v[j];
+                        g[j] *= zz * sigmoid(zz);
+                    }
+                    g[j] = in ? g[j] : 0.f;
+                    d[i][j] = in ? d[i][j] : 0.f;
                 }
+                put_pairs<V>(&sDG[part.row(i)][part.cc], d[i], g);
             }
-            sDG[t][cc] = make_float2(d, g);
-        }
-        stage_bc<T, P>(sC, a.C, a.C_bs, a.C_ts, at.b, at.g, a.N, t0, at.len);
+        });
+        nC.put(sC);
         __syncthreads();
+        if (tile > tile0) next(t0 - SCAN_T);
 #pragma unroll 4
         for (int t = SCAN_T - 1; t >= 0; --t) {
             const float2 dg = sDG[t][c];
-            const float4 c4 = *reinterpret_cast<const float4*>(&sC[t][4 * q]);
-            const float C[4] = {c4.x, c4.y, c4.z, c4.w};
+            float C4[4];
+            load_four(&sC[t][4 * q], C4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lam[i] = (lam[i] + C[i] * dg.y) * __builtin_amdgcn_exp2f(dg.x * A[i]);
+            for (int i = 0; i < 4; ++i) lam[i] = (lam[i] + C4[i] * dg.y) * __builtin_amdgcn_exp2f(dg.x * A[i]);
             total += dg.x;
         }
+        __syncthreads();
     }
     if (!ok) return;
-    store_states(s.xin + ((long long)(at.b * s.nch + at.chunk) * a.D + ch) * (4 * P), 4 * P, q, lam);
+    store_four(s.xin + ((long long)(at.b * s.nch + at.chunk) * a.D + ch) * (4 * P) + 4 * q, lam);
     if (q == 0) s.dsum[(long long)(at.b * s.nch + at.chunk) * a.D + ch] = total;
 }
 
-// Tiles from the last to the first: the states of a tile are recomputed from the one saved before it and stay in registers,
-// then the adjoint runs back through them.
-template <typename T, int P>
-__global__ __launch_bounds__(SCAN_THREADS, P == 1 || P == 16 ? 1 : 2) void scan_bwd_kernel(ScanDev s) {
-    constexpr int CH = SCAN_THREADS / P, NP = 4 * P;
-    __shared__ float2 sDU[SCAN_T][CH];                // delta, u;  afterwards sum_n lam B, sum_n lam h A log2(e)
-    __shared__ float sG[SCAN_T][CH], sY[SCAN_T][CH];
-    __shared__ float sB[SCAN_T][NP], sC[SCAN_T][NP];
-    __shared__ float sP[4][SCAN_T][2 * NP];           // each wave's sums of dB, dC over its channels
+// Sums over a wave's 64 / P channels of the eight values dB[4], dC[4] of every lane.  Lanes trade halves as in sum_steps: after the
+// exchanges across 32, 16 and 8 lanes a lane holds the one value 4 (lane >> 5) + 2 (lane >> 4 & 1) + (lane >> 3 & 1) of its states 4q ..,
+// and the channels that are left (fewer than 8 lanes apart) are added up.  dst: the wave's row [2][4P] of this step.
+__device__ __forceinline__ float trade32(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    const unsigned a = r[0], b = r[1];                // (a bit cast of r[1] itself would read r[0])
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float trade16(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    const unsigned a = r[0], b = r[1];                // (a bit cast of r[1] itself would read r[0])
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+template <int P>
+__device__ __forceinline__ void sum_channels(const float (&p)[8], int lane, int q, float* dst) {
+    float v[4], w[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = trade32(p[i], p[4 + i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = trade16(v[i], v[2 + i]);
+    const int n = 4 * q + 2 * (lane >> 4 & 1);
+    float* out = dst + (lane >> 5) * (4 * P);
+    if constexpr (P == 16) {
+        out[n] = w[0];
+        out[n + 1] = w[1];
+    } else {
+        const bool hi = lane & 8;
+        float r = (hi ? w[1] : w[0]) + dpp<DPP_ROR8>(hi ? w[0] : w[1]);
+        if constexpr (P <= 4) r += dpp<DPP_SHL4>(r);
+        if constexpr (P <= 2) r += dpp<DPP_XOR2>(r);
+        if constexpr (P == 1) r += dpp<DPP_XOR1>(r);
+        if (P == 8 || (lane & 7) < P) out[n + (lane >> 3 & 1)] = r;
+    }
+}
+
+// Tiles of 16 steps from the last to the first: the states and decays of a tile are recomputed from the state saved before it and
+// stay in registers, then the adjoint runs back through them.
+template <typename T, int P, int V>
+__global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_bwd_kernel(ScanDev s) {
+    constexpr int CH = SCAN_THREADS / P, NP = 4 * P, R = SCAN_SAVE, S = Steps<P>::S;
+    __shared__ __attribute__((aligned(16))) float2 sDU[R][CH], sS[R][CH];   // delta, u;  sum_n lam B, sum_n lam h A log2(e)
+    __shared__ __attribute__((aligned(16))) float sG[R][CH], sY[R][CH], sB[R][NP], sC[R][NP];
+    __shared__ float sP[4][R][2 * NP];                // each wave's sums of dB, dC over its channels
     const nmpc_scan_args& a = s.a;
     const ScanPlace<P> at(s);
+    const Part<P, V, R> part;
+    constexpr int PER = Part<P, V, R>::PER;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid / P, q = tid % P, ch = at.c0 + c;
-    const bool ok = c < at.nvalid;
-    float A[4], lam[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, db = 0.f;
+    const bool ok = c < at.nvalid, mine = part.cc < at.nvalid;
+    float A[4], lam[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f}, dD[2] = {0.f, 0.f}, db[2] = {0.f, 0.f}, bias[V], skip[V];
     load_A<P>(s, ch, ok, q, A);
     const long long row = (long long)at.b * s.nch + at.chunk;
     if (ok) {
-        if (s.nch > 1) load_states(s.xin + (row * a.D + ch) * NP, NP, q, lam);
+        if (s.nch > 1) load_four(s.xin + (row * a.D + ch) * NP + 4 * q, lam);
         else if (a.dlast) load_states(a.dlast + ((long long)at.b * a.D + ch) * a.N, a.N, q, lam);
     }
-    const T* u = (const T*)a.u + at.b * a.u_bs + at.c0;
-    const T* dt = (const T*)a.dt + at.b * a.dt_bs + at.c0;
-    const T* z = a.z ? (const T*)a.z + at.b * a.z_bs + at.c0 : nullptr;
-    const T* dy = (const T*)a.dy + at.b * a.dy_bs + at.c0;
-    const long long out0 = (long long)at.b * a.L * a.D + at.c0;
-    const int tile0 = at.chunk * s.tpc, tile1 = min(tile0 + s.tpc, s.ntile);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = a.dt_bias && mine ? a.dt_bias[at.c0 + part.cc + j] : 0.f;
+        skip[j] = a.D_skip && mine ? a.D_skip[at.c0 + part.cc + j] : 0.f;
+    }
+    using PT = Part<P, V, R>;
+    const Stream<T, V, PT> u(a.u, a.u_bs, a.u_ts, at.b, at.c0, part), dt(a.dt, a.dt_bs, a.dt_ts, at.b, at.c0, part),
+        z(a.z, a.z_bs, a.z_ts, at.b, at.c0, part), dy(a.dy, a.dy_bs, a.dy_ts, at.b, at.c0, part);
+    const T* B = (const T*)a.B + at.b * a.B_bs + (long long)at.g * a.N;
+    const T* C = (const T*)a.C + at.b * a.C_bs + (long long)at.g * a.N;
+    auto whole = [&](int t0) { return at.nvalid == CH && t0 + R <= at.len; };
+    const int ntile = (a.L + R - 1) / R, tile0 = at.chunk * s.tpc * (SCAN_T / R), tile1 = min(tile0 + s.tpc * (SCAN_T / R), ntile);
+    Vec<T, V> nd[PER], nu[PER], ng[PER], nz[PER], cd[PER], cg[PER], cz[PER];
+    Shared<T, P, R> nB, nC;
+    auto next = [&](int t0) {
+        whole_or_not(whole(t0), [&](auto w) {
+            dt.template fetch<w.value>(nd, part, t0, at.len, mine);
+            u.template fetch<w.value>(nu, part, t0, at.len, mine);
+            dy.template fetch<w.value>(ng, part, t0, at.len, mine);
+            if (z.p) z.template fetch<w.value>(nz, part, t0, at.len, mine);
+        });
+        nB.fetch(B, a.B_ts, a.N, t0, at.len);
+        nC.fetch(C, a.C_ts, a.N, t0, at.len);
+    };
+    if (tile0 < tile1) next((tile1 - 1) * R);
     for (int tile = tile1 - 1; tile >= tile0; --tile) {
-        const int t0 = tile * SCAN_T;
-        __syncthreads();
-        for (int e = tid; e < SCAN_T * CH; e += SCAN_THREADS) {
-            const int t = e / CH, cc = e % CH;
-            float d = 0.f, uu = 0.f, g = 0.f;
-            if (t0 + t < at.len && cc < at.nvalid) {
-                d = (float)dt[(long long)(t0 + t) * a.dt_ts + cc] + (a.dt_bias ? a.dt_bias[at.c0 + cc] : 0.f);
-                if (a.softplus) d = softplus(d);
-                uu = (float)u[(long long)(t0 + t) * a.u_ts + cc];
-                g = (float)dy[(long long)(t0 + t) * a.dy_ts + cc];
-                if (z) {
-                    const float zz = (float)z[(long long)(t0 + t) * a.z_ts + cc];
-                    g *= zz * sigmoid(zz);
+        const int t0 = tile * R;
+        float x0[4] = {0.f, 0.f, 0.f, 0.f}, xs[R][4], es[R][4];
+        if (ok) load_four((const float*)a.saved + (((long long)at.b * ntile + tile) * a.D + ch) * NP + 4 * q, x0);
+        whole_or_not(whole(t0), [&](auto w) {
+            float d[PER][V];
+            deltas(d, nd, bias, a.softplus);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const bool in = w.value || (mine && t0 + part.row(i) < at.len);
+                float uu[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float g = (float)ng[i].v[j];
+                    if (z.p) {
+                        const float zz = (float)nz[i].v[j];
+                        g *= zz * sigmoid(zz);
+                    }
+                    uu[j] = in ? (float)nu[i].v[j] : 0.f;
+                    d[i][j] = in ? d[i][j] : 0.f;
+                    sG[part.row(i)][part.cc + j] = in ? g : 0.f;
                 }
+                put_pairs<V>(&sDU[part.row(i)][part.cc], d[i], uu);
+                cd[i] = nd[i]; cg[i] = ng[i]; cz[i] = nz[i];
             }
-            sDU[t][cc] = make_float2(d, uu);
-            sG[t][cc] = g;
-        }
-        stage_bc<T, P>(sB, a.B, a.B_bs, a.B_ts, at.b, at.g, a.N, t0, at.len);
-        stage_bc<T, P>(sC, a.C, a.C_bs, a.C_ts, at.b, at.g, a.N, t0, at.len);
-        float x0[4] = {0.f, 0.f, 0.f, 0.f}, xs[SCAN_T][4];
-        if (ok) load_states((const float*)a.saved + (((long long)at.b * s.ntile + tile) * a.D + ch) * NP, NP, q, x0);
+        });
+        nB.put(sB);
+        nC.put(sC);
         __syncthreads();
+        if (tile > tile0) next(t0 - R);
 #pragma unroll
-        for (int t = 0; t < SCAN_T; ++t) {
-            const float2 du = sDU[t][c];
-            const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][4 * q]);
-            const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+        for (int t4 = 0; t4 < R; t4 += S) {
+            float y[S];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                xs[t][i] = __builtin_amdgcn_exp2f(du.x * A[i]) * (t ? xs[t - 1][i] : x0[i]) + (du.x * du.y) * b[i];
-            if (z) {
-                const float4 c4 = *reinterpret_cast<const float4*>(&sC[t][4 * q]);
-                const float y = sum_lanes<P>(c4.x * xs[t][0] + c4.y * xs[t][1] + c4.z * xs[t][2] + c4.w * xs[t][3]);
-                if (q == 0) sY[t][c] = y;
-            }
-        }
-#pragma unroll
-        for (int t = SCAN_T - 1; t >= 0; --t) {
-            const float2 du = sDU[t][c];
-            const float g = sG[t][c], w = du.x * du.y;
-            const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][4 * q]), c4 = *reinterpret_cast<const float4*>(&sC[t][4 * q]);
-            const float b[4] = {b4.x, b4.y, b4.z, b4.w}, C[4] = {c4.x, c4.y, c4.z, c4.w};
-            float s1 = 0.f, s2 = 0.f, p[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(du.x * A[i]);
-                lam[i] += C[i] * g;
-                p[i] = lam[i] * w;
-                p[4 + i] = xs[t][i] * g;
-                s1 += lam[i] * b[i];
-                lam[i] *= e;
-                const float m = lam[i] * (t ? xs[t > 0 ? t - 1 : 0][i] : x0[i]);
-                s2 += m * A[i];
-                dA[i] += m * du.x;
-            }
-            s1 = sum_lanes<P>(s1);
-            s2 = sum_lanes<P>(s2);
-            // all lanes of the channel have read this entry (they are in one wave)
-            if (q == 0) sDU[t][c] = make_float2(s1, s2);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-#pragma unroll
-                for (int m = P; m < 64; m *= 2) p[i] += __shfl_xor(p[i], m);
-            }
-            if (lane < P) {
+            for (int k = 0; k < S; ++k) {
+                const int t = t4 + k;
+                const float2 du = sDU[t][c];
+                const float w = du.x * du.y;
+                float b[4];
+                load_four(&sB[t][4 * q], b);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sP[wave][t][4 * q + i] = p[i];
-                    sP[wave][t][NP + 4 * q + i] = p[4 + i];
+                    es[t][i] = __builtin_amdgcn_exp2f(du.x * A[i]);
+                    xs[t][i] = es[t][i] * (t ? xs[t ? t - 1 : 0][i] : x0[i]) + w * b[i];
+                }
+                if (z.p) {
+                    float C4[4];
+                    load_four(&sC[t][4 * q], C4);
+                    y[k] = C4[0] * xs[t][0] + C4[1] * xs[t][1] + C4[2] * xs[t][2] + C4[3] * xs[t][3];
                 }
             }
+            if (z.p) {
+                const float r = sum_steps<P>(y, tid);
+                if (P <= 4 || q < 4) sY[t4 + (q & 3)][c] = r;
+            }
+        }
+#pragma unroll
+        for (int t4 = R - S; t4 >= 0; t4 -= S) {
+            float s1[S], s2[S];
+#pragma unroll
+            for (int k = S - 1; k >= 0; --k) {
+                const int t = t4 + k;
+                const float2 du = sDU[t][c];
+                const float g = sG[t][c], w = du.x * du.y;
+                float b[4], C4[4], p[8];
+                load_four(&sB[t][4 * q], b);
+                load_four(&sC[t][4 * q], C4);
+                s1[k] = s2[k] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    lam[i] += C4[i] * g;
+                    p[i] = lam[i] * w;
+                    p[4 + i] = xs[t][i] * g;
+                    s1[k] += lam[i] * b[i];
+                    lam[i] *= es[t][i];
+                    const float m = lam[i] * (t ? xs[t ? t - 1 : 0][i] : x0[i]);
+                    s2[k] += m * A[i];
+                    dA[i] += m * du.x;
+                }
+                sum_channels<P>(p, lane, q, sP[wave][t]);
+            }
+            const float r1 = sum_steps<P>(s1, tid), r2 = sum_steps<P>(s2, tid);
+            if (P <= 4 || q < 4) sS[t4 + (q & 3)][c] = make_float2(r1, r2);
         }
         __syncthreads();
-        for (int e = tid; e < SCAN_T * 2 * NP; e += SCAN_THREADS) {
+        const long long blk = (at.c0 - at.g * s.per) / CH;
+        for (int e = tid; e < R * 2 * NP; e += SCAN_THREADS) {
             const int t = e / (2 * NP), n = e % (2 * NP);
-            if (t0 + t >= a.L) continue;
-            const float v = (sP[0][t][n] + sP[1][t][n]) + (sP[2][t][n] + sP[3][t][n]);
-            const long long blk = (at.c0 - at.g * s.per) / CH;
-            s.pBC[(((blk * a.nb + at.b) * a.L + t0 + t) * a.G + at.g) * (2 * NP) + n] = v;
+            if (t0 + t < a.L)
+                s.pBC[(((blk * a.nb + at.b) * a.L + t0 + t) * a.G + at.g) * (2 * NP) + n] = (sP[0][t][n] + sP[1][t][n]) + (sP[2][t][n] + sP[3][t][n]);
         }
-        for (int e = tid; e < SCAN_T * CH; e += SCAN_THREADS) {
-            const int t = e / CH, cc = e % CH;
-            if (t0 + t >= a.L || cc >= at.nvalid) continue;
-            const long long o = out0 + (long long)(t0 + t) * a.D + cc;
-            float vu = 0.f, vd = 0.f, vz = 0.f;
-            if (t0 + t < at.len) {
-                const float2 sums = sDU[t][cc];
-                const float raw = (float)dt[(long long)(t0 + t) * a.dt_ts + cc] + (a.dt_bias ? a.dt_bias[at.c0 + cc] : 0.f);
-                const float d = a.softplus ? softplus(raw) : raw, uu = (float)u[(long long)(t0 + t) * a.u_ts + cc], g = sG[t][cc];
-                const float skip = a.D_skip ? a.D_skip[at.c0 + cc] : 0.f;
-                vu = skip * g + d * sums.x;
-                vd = sums.y * (1.f / LOG2E) + uu * sums.x;
-                if (a.softplus) vd *= sigmoid(raw);
-                if (z) {
-                    const float zz = (float)z[(long long)(t0 + t) * a.z_ts + cc], p = sigmoid(zz);
-                    vz = (float)dy[(long long)(t0 + t) * a.dy_ts + cc] * (sY[t][cc] + skip * uu) * (p * (1.f + zz * (1.f - p)));
+        const long long out = ((long long)at.b * a.L + t0) * a.D + at.c0;
+        whole_or_not(whole(t0), [&](auto w) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int t = part.row(i);
+                if (!w.value && (!mine || t0 + t >= a.L)) continue;
+                const bool in = w.value || t0 + t < at.len;
+                Vec<T, V> ou, od, oz;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float2 sums = sS[t][part.cc + j], du = sDU[t][part.cc + j];      // zero past the sequence, as is g
+                    const float g = sG[t][part.cc + j];
+                    const float vu = skip[j] * g + du.x * sums.x;
+                    float vd = sums.y * (1.f / LOG2E) + du.y * sums.x, vz = 0.f;
+                    if (a.softplus) vd *= sigmoid((float)cd[i].v[j] + bias[j]);
+                    if (z.p) {
+                        const float zz = (float)cz[i].v[j], p = sigmoid(zz);
+                        vz = (float)cg[i].v[j] * (sY[t][part.cc + j] + skip[j] * du.y) * (p * (1.f + zz * (1.f - p)));
+                    }
+                    ou.v[j] = (T)(in ? vu : 0.f); od.v[j] = (T)(in ? vd : 0.f); oz.v[j] = (T)(in ? vz : 0.f);
+                    if (in) {
+                        dD[V == 2 ? j : i & 1] += g * du.y;
+                        db[V == 2 ? j : i & 1] += vd;
+                    }
                 }
-                dD += g * uu;
-                db += vd;
+                const long long o = out + (long long)(i * PT::STEP) * a.D + (unsigned)(part.t * a.D + part.cc);
+                store_vec((T*)a.du + o, ou);
+                store_vec((T*)a.ddt + o, od);
+                if (z.p) store_vec((T*)a.dz + o, oz);
             }
-            ((T*)a.du)[o] = (T)vu;
-            ((T*)a.ddt)[o] = (T)vd;
-            if (z) ((T*)a.dz)[o] = (T)vz;
-        }
+        });
+        __syncthreads();                              // sG, sDU and sP are written again
     }
     if (ok) {
-        store_states(s.pA + (row * a.D + ch) * NP, NP, q, dA);
+        store_four(s.pA + (row * a.D + ch) * NP + 4 * q, dA);
         if (a.dstart && at.chunk == 0) store_states(a.dstart + ((long long)at.b * a.D + ch) * a.N, a.N, q, lam);
     }
-    // dD and the bias: a thread's elements are all of channel tid % CH
-    __syncthreads();
-    float* red = &sG[0][0];
-    red[tid] = dD;
-    red[SCAN_THREADS + tid] = db;
+    // dD and the bias, joined over the threads that share channels.  A thread has two sums each: of two channels (V = 2), or of its even
+    // and odd rows (V = 1), so that the order of additions, and with it the result, is the same for both.
+    constexpr int COLS = Part<P, V, R>::COLS, STEP = Part<P, V, R>::STEP, CLASSES = V == 2 || PER == 1 ? STEP : 2 * STEP;
+    float* red = &sDU[0][0].x;
+    static_assert(sizeof(sDU) >= 4 * SCAN_THREADS * sizeof(float) || (V == 1 && PER == 1), "reduction buffer");
+#pragma unroll
+    for (int j = 0; j < (V == 2 || PER > 1 ? 2 : 1); ++j) {
+        red[(2 * j) * SCAN_THREADS + tid] = dD[j];
+        red[(2 * j + 1) * SCAN_THREADS + tid] = db[j];
+    }
     __syncthreads();
     if (tid < at.nvalid) {
         float v0 = 0.f, v1 = 0.f;
-        for (int r = tid; r < SCAN_THREADS; r += CH) { v0 += red[r]; v1 += red[SCAN_THREADS + r]; }
+        for (int k = 0; k < CLASSES; ++k) {
+            const int j = V == 2 ? tid & 1 : k / STEP, r = (V == 2 ? k : k % STEP) * COLS + tid / V;
+            v0 += red[(2 * j) * SCAN_THREADS + r];
+            v1 += red[(2 * j + 1) * SCAN_THREADS + r];
+        }
         s.pDb[(row * 2) * a.D + at.c0 + tid] = v0;
         s.pDb[(row * 2 + 1) * a.D + at.c0 + tid] = v1;
     }
@@ -481,6 +749,21 @@ static void scan_plan(ScanDev& s) {
     s.ntile = a.L > 0 ? (a.L + SCAN_T - 1) / SCAN_T : 0;
     s.nch = 1;
     s.tpc = s.ntile;
+    const long long base = (long long)a.nb * a.G * s.nblk;
+    const int target = 1024;           // workgroups: four a CU
+    if (base > 0 && base * 2 <= target && s.ntile > 1) {
+        const long long want = (target + base - 1) / base;
+        const int n = want < s.ntile ? (int)want : s.ntile;
+        s.tpc = (s.ntile + n - 1) / n;
+        s.nch = (s.ntile + s.tpc - 1) / s.tpc;
+    }
+}
+
+// may the samples be accessed in pairs of channels?
+template <typename T>
+static bool scan_pairs(const ScanDev& s) {
+    const nmpc_scan_args& a = s.a;
+    return s.per % 2 == 0 && vec_ok<T>(a.u, a.u_bs, a.u_ts, 2) && vec_ok<T>(a.dt, a.dt_bs, a.dt_ts, 2) && vec_ok<T>(a.z, a.z_bs, a.z_ts, 2);
 }
 
 static unsigned long long round256(unsigned long long v) { return (v + 255) / 256 * 256; }
@@ -511,6 +794,10 @@ static int scan_check(const char* what, const nmpc_scan_args* a) {
     // a launch has fewer than 2^32 threads
     NMPC_REQUIRE((long long)a->nb * a->D * 64 < (1ll << 31) && (long long)a->nb * (a->D / 16 + a->G) * (a->L / SCAN_T + 1) < (1ll << 23),
                  "%s: too many elements for one launch", what);
+    // a thread's offset within 16 rows is kept in 32 bits
+    const long long most = 1ll << 24;
+    NMPC_REQUIRE(a->D <= most && a->u_ts >= 0 && a->u_ts <= most && a->dt_ts >= 0 && a->dt_ts <= most && (!a->z || (a->z_ts >= 0 && a->z_ts <= most)) &&
+                 (!a->dy || (a->dy_ts >= 0 && a->dy_ts <= most)), "%s: strides between steps of 0..2^24 elements", what);
     return 0;
 }
 
@@ -529,7 +816,7 @@ using namespace nmpc;
 
 extern "C" unsigned long long nmpc_lpv_scan_saved_bytes(int nb, int L, int D, int N) {
     if (nb <= 0 || L <= 0 || D <= 0 || N <= 0 || N > 64) return 0;
-    return (unsigned long long)nb * ((L + SCAN_T - 1) / SCAN_T) * D * 4 * scan_lanes(N) * sizeof(float);
+    return (unsigned long long)nb * ((L + SCAN_SAVE - 1) / SCAN_SAVE) * D * 4 * scan_lanes(N) * sizeof(float);
 }
 
 extern "C" unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D, int N, int G, int backward) {
@@ -554,11 +841,15 @@ extern "C" int nmpc_lpv_scan(const nmpc_scan_args* args, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
+            constexpr int V_ = P_ == 16 ? 1 : 2;          // 16 channels: fewer pairs than a tile has rows for
+            const bool pairs = scan_pairs<T_>(s) && vec_ok<T_>(a.y, 0, 0, 2);
             if (s.nch > 1) {
-                scan_fwd_kernel<T_, P_, true><<<grid, SCAN_THREADS, 0, st>>>(s);
+                if (pairs) scan_fwd_kernel<T_, P_, V_, true><<<grid, SCAN_THREADS, 0, st>>>(s);
+                else scan_fwd_kernel<T_, P_, 1, true><<<grid, SCAN_THREADS, 0, st>>>(s);
                 scan_chunks_kernel<false><<<(unsigned)(((long long)a.nb * a.D * 4 * P_ + 255) / 256), 256, 0, st>>>(s, 4 * P_);
             }
-            scan_fwd_kernel<T_, P_, false><<<grid, SCAN_THREADS, 0, st>>>(s);
+            if (pairs) scan_fwd_kernel<T_, P_, V_, false><<<grid, SCAN_THREADS, 0, st>>>(s);
+            else scan_fwd_kernel<T_, P_, 1, false><<<grid, SCAN_THREADS, 0, st>>>(s);
         })
     })
     NMPC_HIP_CHECK(hipGetLastError());
@@ -582,13 +873,17 @@ extern "C" int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
-            constexpr int NP = 4 * P_;
+            constexpr int NP = 4 * P_, V_ = P_ == 16 ? 1 : 2;
             if (a.nb > 0) {
+                const bool pairs = scan_pairs<T_>(s) && vec_ok<T_>(a.dy, a.dy_bs, a.dy_ts, 2) && vec_ok<T_>(a.du, 0, 0, 2) &&
+                                   vec_ok<T_>(a.ddt, 0, 0, 2) && vec_ok<T_>(a.dz, 0, 0, 2);
                 if (s.nch > 1) {
-                    scan_bwd_summary_kernel<T_, P_><<<grid, SCAN_THREADS, 0, st>>>(s);
+                    if (pairs) scan_bwd_summary_kernel<T_, P_, V_><<<grid, SCAN_THREADS, 0, st>>>(s);
+                    else scan_bwd_summary_kernel<T_, P_, 1><<<grid, SCAN_THREADS, 0, st>>>(s);
                     scan_chunks_kernel<true><<<(unsigned)(((long long)a.nb * a.D * NP + 255) / 256), 256, 0, st>>>(s, NP);
                 }
-                scan_bwd_kernel<T_, P_><<<grid, SCAN_THREADS, 0, st>>>(s);
+                if (pairs) scan_bwd_kernel<T_, P_, V_><<<grid, SCAN_THREADS, 0, st>>>(s);
+                else scan_bwd_kernel<T_, P_, 1><<<grid, SCAN_THREADS, 0, st>>>(s);
             }
             scan_reduce_params_kernel<<<(unsigned)(((long long)a.D * (NP + 2) + 255) / 256), 256, 0, st>>>(s, NP);
             const long long nbc = (long long)a.nb * a.L * a.G * 2 * NP;

@@ -4,6 +4,8 @@
 // Both projections of a tile are accumulated side by side, so that the activation and the product happen in registers and
 // neither projection is written (a training pass keeps both in fp32 for the gradient).  Products run on the matrix cores with
 // fp32 accumulation; dG and dU are rounded to the element type once, as operands of the next products.
+#include <cmath>
+
 #include "seq_common.h"
 
 namespace nmpc {
@@ -30,13 +32,15 @@ __device__ __forceinline__ float2 activation(int act, float x) {
 }
 
 // ---- products of many rows -------------------------------------------------------------------------------------------
-// out[m][n] = sum_k A[m][k] B[n][k], both operands with contiguous rows of whole 128-byte k-tiles.
+// out[m][n] = sum_k A(m,k) B(n,k).  An operand is stored either with k contiguous (rows of whole 64-byte pieces) or with its own index
+// contiguous (row k holds all m or n; up to kmax rows, a multiple of 16 bytes each).
 struct NtArgs {
-    const void *A, *B, *B1;            // GATED: B and B1 are the two weight matrices
+    const void *A, *B, *B1;            // GATED: B, B1 are the two weight matrices, side by side in n.  B stored by k: B holds k < kcut, B1 the rest
     long long a_ld, b_ld;              // elements
     int M, N, ktiles, act;
-    void *out, *out1;                  // rows from `cut` on go to out1 (two gradients of one product)
-    int cut;
+    int kcut, a_kmax, b_kmax;          // operands stored by k: rows of each part that exist (past them the other operand is zero)
+    void *out, *out1;                  // rows from `cut` on go to out1 (two gradients of one product); `rows` rows of each exist
+    int cut, rows;
     float* pre;                        // GATED: [2][M][N], both projections, may be null
     float* part;                       // fp32 partial products [splits][M][N] instead of out
     int splits;
@@ -87,16 +91,52 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int left, bool
     }
 }
 
+// 16 bytes (8 or 4 steps of k) of an operand's fragment: rows base + (lane & 31) of the tile, k pieces 2 ks + (lane >> 5)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <typename T, int ROWS, bool KC>
+struct Fragment {
+    int off;                           // of this lane, for rows base ..
+    __device__ __forceinline__ Fragment(int base, int lane) {
+        if constexpr (KC) off = (base + (lane & 31)) * 64;
+        else if constexpr (sizeof(T) == 2) {
+            const int k3 = (lane >> 2) & 3;
+            off = ((lane >> 5) * 8 + k3) * (ROWS * 2) + ((base / 8) ^ (k3 << 2)) * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        } else off = (lane >> 5) * 4 * (ROWS * 4) + (base + (lane & 31)) * 4;
+    }
+    __device__ __forceinline__ uint4 read(const char* buf, int ks, int lane) const {
+        if constexpr (KC) {
+            return *reinterpret_cast<const uint4*>(buf + off + ((ks * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16);
+        } else if constexpr (sizeof(T) == 2) {
+            // a transposing read: 16 lanes give the addresses of 4 rows k of 16 columns and get 4 steps of k of a column each
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const char* p = buf + off + ks * 16 * (ROWS * 2);
+            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * ROWS * 2)));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+            const char* p = buf + off + ks * 8 * (ROWS * 4);
+            uint4 v;
+            v.x = *reinterpret_cast<const unsigned*>(p);
+            v.y = *reinterpret_cast<const unsigned*>(p + ROWS * 4);
+            v.z = *reinterpret_cast<const unsigned*>(p + 2 * ROWS * 4);
+            v.w = *reinterpret_cast<const unsigned*>(p + 3 * ROWS * 4);
+            return v;
+        }
+    }
+};
+
 // WM x WN waves; a wave owns MI x 2 accumulators of 32 x 32: rows 32 MI wm .., columns 32 wn .. and BN / 2 + 32 wn .. (GATED: the same
-// hidden units of both projections).  A k-tile is a row of 128 bytes, moved from global memory to LDS without passing through
-// registers, into two buffers in turn: the loads of the next tile are in flight while this one is multiplied.  Within a row the
-// 16-byte pieces sit at piece ^ (row & 7), so that the 8 rows that a read serves at once touch all banks.
-template <typename T, int WM, int WN, int MI, bool GATED>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_nt_kernel(NtArgs g) {
-    constexpr int BM = WM * MI * 32, BN = WN * 64, WAVES = WM * WN, ROWS = BM + BN, LOADS = ROWS / 8 / WAVES;
-    static_assert(ROWS % (8 * WAVES) == 0 && BM % 8 == 0, "whole loads");
-    // two objects, not one array: the compiler then knows that reads of one do not wait for loads into the other
-    __shared__ __attribute__((aligned(1024))) char lds0[ROWS * 128], lds1[ROWS * 128];
+// hidden units of both projections).  A k-tile is 64 bytes deep (32 or 16 steps).  It moves from global memory to LDS without passing
+// through registers, into four buffers in turn: the loads of three tiles are in flight while one is multiplied, one barrier a tile.
+// With two buffers of twice the depth the product waited for its loads most of the time (0.89 PFLOP/s at 4096 x 2048 x 16384).
+// Pieces of 16 bytes are stored at places exclusive-ored with the row, so that the rows that a read serves at once touch all banks.
+template <typename T, int WM, int WN, int MI, bool GATED, bool KA, bool KB>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
+    constexpr int BM = WM * MI * 32, BN = WN * 64, WAVES = WM * WN, E = 16 / sizeof(T), BK = 64 / sizeof(T);
+    constexpr int LOADS = (BM + BN) * 64 / 1024 / WAVES, AUNITS = BM / 16;
+    static_assert((BM + BN) * 64 % (1024 * WAVES) == 0 && AUNITS % WAVES == 0 && (!GATED || (KA && KB)), "whole loads");
+    // separate objects, not one array: the compiler then knows that reads of one do not wait for loads into the others
+    __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * 64], lds1[(BM + BN) * 64], lds2[(BM + BN) * 64], lds3[(BM + BN) * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // consecutive workgroups go to the 8 dies in turn: give each die a contiguous part of the tiles, walked 8 rows of tiles deep
     int id = blockIdx.x;
@@ -112,67 +152,122 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_nt_kernel(NtArgs g) {
     const int n0 = nt * (GATED ? BN / 2 : BN);
     const int kt0 = (int)((long long)g.ktiles * split / g.splits), kt1 = (int)((long long)g.ktiles * (split + 1) / g.splits);
 
+    // load i of a wave fills 1 KB: 16 rows of 64 bytes (k contiguous), or rows k of BM or BN elements
     const char* src[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int row = (i * WAVES + wave) * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
-        const char* p;
-        if (row < BM) {
-            p = (const char*)g.A + (long long)min(m0 + row, g.M - 1) * g.a_ld * sizeof(T);
-        } else {                       // rows past the end repeat the last one; their results are not stored
-            const int r = row - BM;
-            if (GATED) p = (const char*)(r < BN / 2 ? g.B : g.B1) + (long long)min(n0 + r % (BN / 2), g.N - 1) * g.b_ld * sizeof(T);
-            else p = (const char*)g.B + (long long)min(n0 + r, g.N - 1) * g.b_ld * sizeof(T);
+        const int unit = i * WAVES + wave;
+        if (i * WAVES < AUNITS) {
+            if constexpr (KA) {
+                const int row = unit * 16 + (lane >> 2), piece = (lane & 3) ^ (lane >> 4);
+                src[i] = (const char*)g.A + (long long)min(m0 + row, g.M - 1) * g.a_ld * sizeof(T) + piece * 16;
+            } else {
+                constexpr int RB = BM * sizeof(T);
+                const int k = (unit * 1024 + lane * 16) / RB, piece = (lane * 16 % RB) / 16 ^ (sizeof(T) == 2 ? (k & 3) << 2 : 0);
+                src[i] = (const char*)g.A + min(m0 + piece * E, (g.M - 1) / E * E) * sizeof(T);
+            }
+        } else {
+            const int ub = unit - AUNITS;
+            if constexpr (KB) {
+                const int r = ub * 16 + (lane >> 2), piece = (lane & 3) ^ (lane >> 4);
+                const char* p;                                    // rows past the end repeat the last one; their results are not stored
+                if (GATED) p = (const char*)(r < BN / 2 ? g.B : g.B1) + (long long)min(n0 + r % (BN / 2), g.N - 1) * g.b_ld * sizeof(T);
+                else p = (const char*)g.B + (long long)min(n0 + r, g.N - 1) * g.b_ld * sizeof(T);
+                src[i] = p + piece * 16;
+            } else {
+                constexpr int RB = BN * sizeof(T);
+                const int k = (ub * 1024 + lane * 16) / RB, piece = (lane * 16 % RB) / 16 ^ (sizeof(T) == 2 ? (k & 3) << 2 : 0);
+                src[i] = (const char*)(unsigned long long)(min(n0 + piece * E, (g.N - 1) / E * E) * sizeof(T));
+            }
         }
-        src[i] = p + piece * 16 + (long long)kt0 * 128;
     }
-    auto issue = [&](char* buf) {
+    auto issue = [&](char* buf, int kt) {
+        kt = min(kt, kt1 - 1);         // past the end the last tile again, so that the number of loads in flight stays the same
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
-                                             (__attribute__((address_space(3))) void*)(buf + (i * WAVES + wave) * 1024), 16, 0, 0);
-            src[i] += 128;
+            const int unit = i * WAVES + wave;
+            const char* p;
+            if (i * WAVES < AUNITS) {
+                if constexpr (KA) p = src[i] + (long long)kt * 64;
+                else p = src[i] + (long long)min(kt * BK + (unit * 1024 + lane * 16) / (int)(BM * sizeof(T)), g.a_kmax - 1) * g.a_ld * sizeof(T);
+            } else {
+                if constexpr (KB) p = src[i] + (long long)kt * 64;
+                else {
+                    const bool second = kt * BK >= g.kcut;
+                    const int k = kt * BK - (second ? g.kcut : 0) + ((unit - AUNITS) * 1024 + lane * 16) / (int)(BN * sizeof(T));
+                    p = (const char*)(second ? g.B1 : g.B) + (unsigned long long)src[i] + (long long)min(k, g.b_kmax - 1) * g.b_ld * sizeof(T);
+                }
+            }
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                             (__attribute__((address_space(3))) void*)(buf + unit * 1024), 16, 0, 0);
         }
     };
     f32x16 acc[MI][2] = {};
     auto multiply = [&](const char* buf) {
-        const char* a = buf + (wm * MI * 32 + (lane & 31)) * 128;
-        const char* b = buf + (BM + wn * 32 + (lane & 31)) * 128;
+        const Fragment<T, BN, KB> fb0(wn * 32, lane), fb1(BN / 2 + wn * 32, lane);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const int piece = ((ks * 2 + (lane >> 5)) ^ (lane & 7)) * 16;
-            const uint4 b0 = *reinterpret_cast<const uint4*>(b + piece), b1 = *reinterpret_cast<const uint4*>(b + BN / 2 * 128 + piece);
+        for (int ks = 0; ks < 2; ++ks) {
+            const uint4 b0 = fb0.read(buf + BM * 64, ks, lane), b1 = fb1.read(buf + BM * 64, ks, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                const uint4 av = *reinterpret_cast<const uint4*>(a + i * 32 * 128 + piece);
+                const Fragment<T, BM, KA> fa((wm * MI + i) * 32, lane);
+                const uint4 av = fa.read(buf, ks, lane);
                 acc[i][0] = Mma<T>::step(av, b0, acc[i][0]);
                 acc[i][1] = Mma<T>::step(av, b1, acc[i][1]);
             }
         }
     };
-    // before a tile is read: its loads (counted as memory loads) have arrived, and everyone is done with the other buffer
+    // before a tile is read: its loads have arrived (two tiles' may still be in flight), everyone's have, and everyone has read the
+    // tile whose buffer is filled next
     auto arrive = [] {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        static_assert(LOADS == 4, "loads that may be in flight: two tiles");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0078);            // vmcnt 8, lgkmcnt 0; as a builtin, so that the compiler counts with it
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
-    if (kt0 < kt1) issue(lds0);
+    if (kt0 < kt1) {
+        issue(lds0, kt0);
+        issue(lds1, kt0 + 1);
+        issue(lds2, kt0 + 2);
+    }
     int kt = kt0;
-    for (; kt + 2 <= kt1; kt += 2) {
+    for (; kt + 4 <= kt1; kt += 4) {
         arrive();
-        issue(lds1);
+        issue(lds3, kt + 3);
         multiply(lds0);
         arrive();
-        if (kt + 2 < kt1) issue(lds0);
+        issue(lds0, kt + 4);
         multiply(lds1);
+        arrive();
+        issue(lds1, kt + 5);
+        multiply(lds2);
+        arrive();
+        issue(lds2, kt + 6);
+        multiply(lds3);
     }
     if (kt < kt1) {
         arrive();
+        issue(lds3, kt + 3);           // (not read: keeps the count)
         multiply(lds0);
+        if (kt + 1 < kt1) {
+            arrive();
+            issue(lds0, kt + 4);
+            multiply(lds1);
+            if (kt + 2 < kt1) {
+                arrive();
+                multiply(lds2);
+            }
+        }
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);                // nothing in flight
     __syncthreads();
     // Results: 32 rows at a time through 8 KB of LDS of the wave's own, so that a lane has 8 neighbouring columns; 4-column pieces sit
     // at piece ^ (row & 15) against bank conflicts.
-    float* stage = reinterpret_cast<float*>(lds0) + wave * 2048;
+    constexpr int PER = (BM + BN) * 64 / 8192;
+    static_assert(2 * PER >= WAVES, "room for the results");
+    float* stage = reinterpret_cast<float*>(wave < PER ? lds0 : lds1) + (wave % PER) * 2048;
     const bool wide = g.N % 8 == 0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -212,8 +307,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_nt_kernel(NtArgs g) {
                 for (int c = 0; c < 2; ++c) {
                     const int n = n0 + c * (BN / 2) + wn * 32 + q * 8;
                     if (g.part) store8(g.part + ((long long)split * g.M + m) * g.N + n, v[c], g.N - n, wide);
-                    else if (m < g.cut) store8((T*)g.out + (long long)m * g.N + n, v[c], g.N - n, wide);
-                    else store8((T*)g.out1 + (long long)(m - g.cut) * g.N + n, v[c], g.N - n, wide);
+                    else if (m < g.cut ? m < g.rows : m - g.cut < g.rows)
+                        store8((T*)(m < g.cut ? g.out : g.out1) + (long long)(m < g.cut ? m : m - g.cut) * g.N + n, v[c], g.N - n, wide);
                 }
             }
         }
@@ -224,12 +319,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_nt_kernel(NtArgs g) {
 // out = sum of the splits' partial products, in order
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(NtArgs g) {
-    const long long total = (long long)g.M * g.N, cut = (long long)g.cut * g.N;
+    const long long total = (long long)g.M * g.N;
     for (long long o = (long long)blockIdx.x * 256 + threadIdx.x; o < total; o += 256ll * gridDim.x) {
         float v = 0.f;
         for (int k = 0; k < g.splits; ++k) v += g.part[k * total + o];
-        if (o < cut) ((T*)g.out)[o] = (T)v;
-        else ((T*)g.out1)[o - cut] = (T)v;
+        const int m = (int)(o / g.N), r = m < g.cut ? m : m - g.cut;
+        if (r < g.rows) ((T*)(m < g.cut ? g.out : g.out1))[(long long)r * g.N + o % g.N] = (T)v;
     }
 }
 
@@ -351,48 +446,46 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long long s_ld, 
     }
 }
 
-// dst[c][at + r] = src[r][c]; columns at + rows .. at + ld_rows of dst are cleared
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T* src, long long s_ld, int rows, int cols, T* dst, long long d_ld, int padded) {
-    __shared__ T tile[64][65];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int r = y; r < 64; r += 4) tile[r][x] = r0 + r < rows && c0 + x < cols ? src[(long long)(r0 + r) * s_ld + c0 + x] : (T)0.f;
-    __syncthreads();
-    for (int c = y; c < 64; c += 4)
-        if (c0 + c < cols && r0 + x < padded) dst[(long long)(c0 + c) * d_ld + r0 + x] = tile[x][c];
-}
-
-// dG, dU from the saved projections: rows [M][2 Fp] (dG, then dU, each zero from F on) for the product with the weights, and
-// transposed [2 F][Mp] (zero from M on) for the product with x.
-template <typename T>
-__global__ __launch_bounds__(256) void gate_slope_kernel(int M, int F, int Mp, int Fp, int act, const float* pre, const T* dh, long long dh_ld,
-                                                         T* rows, T* cols) {
-    __shared__ T tile[2][64][65];
-    const int m0 = blockIdx.x * 64, f0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    const long long total = (long long)M * F;
-    for (int r = y; r < 64; r += 4) {
-        const int m = m0 + r, f = f0 + x;
-        T vg = (T)0.f, vu = (T)0.f;
-        if (m < M && f < F) {
-            const long long o = (long long)m * F + f;
-            const float d = (float)dh[(long long)m * dh_ld + f];
-            const float2 a = activation(act, pre[o]);
-            vg = (T)(d * pre[total + o] * a.y);
-            vu = (T)(d * a.x);
+// dG, dU from the saved projections: rows [Mp][2 Fp], dG then dU, zero past M and past F.  Bound by memory (2 e + 2 e + 8 + e bytes an
+// element): eight elements a thread; VEC: rows of pre and dh may be read in pieces of 16 bytes.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void gate_slope_kernel(int M, int F, int Mp, int Fp, int act, const float* pre, const T* dh, long long dh_ld, T* rows) {
+    constexpr int E = 16 / sizeof(T);
+    const unsigned cols = Fp / 8, m = blockIdx.x / ((cols + 255) / 256), c = blockIdx.x % ((cols + 255) / 256) * 256 + threadIdx.x;
+    if (c >= cols) return;
+    const int f = c * 8;
+    const long long o = (long long)m * F + f, total = (long long)M * F;
+    float g[8], u[8];
+    T d[8], vg[8], vu[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { g[i] = u[i] = 0.f; d[i] = (T)0.f; }
+    if ((int)m < M) {
+        if constexpr (VEC) {
+            if (f < F) {               // F is a multiple of 8
+                *(float4*)g = *(const float4*)(pre + o); *(float4*)(g + 4) = *(const float4*)(pre + o + 4);
+                *(float4*)u = *(const float4*)(pre + total + o); *(float4*)(u + 4) = *(const float4*)(pre + total + o + 4);
+#pragma unroll
+                for (int i = 0; i < 8; i += E) *(Vec<T, E>*)(d + i) = load_vec<T, E>(dh + (long long)m * dh_ld + f + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (f + i < F) { g[i] = pre[o + i]; u[i] = pre[total + o + i]; d[i] = dh[(long long)m * dh_ld + f + i]; }
         }
-        if (m < M && f < Fp) {
-            rows[(long long)m * 2 * Fp + f] = vg;
-            rows[(long long)m * 2 * Fp + Fp + f] = vu;
-        }
-        tile[0][r][x] = vg;
-        tile[1][r][x] = vu;
     }
-    __syncthreads();
-    for (int c = y; c < 64; c += 4)
-        if (f0 + c < F && m0 + x < Mp) {
-            cols[(long long)(f0 + c) * Mp + m0 + x] = tile[0][x][c];
-            cols[(long long)(F + f0 + c) * Mp + m0 + x] = tile[1][x][c];
-        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 a = activation(act, g[i]);
+        const bool in = (int)m < M && f + i < F;
+        vg[i] = (T)(in ? (float)d[i] * u[i] * a.y : 0.f);
+        vu[i] = (T)(in ? (float)d[i] * a.x : 0.f);
+    }
+    T* out = rows + (long long)m * 2 * Fp + f;
+#pragma unroll
+    for (int i = 0; i < 8; i += E) {
+        store_vec(out + i, *(const Vec<T, E>*)(vg + i));
+        store_vec(out + Fp + i, *(const Vec<T, E>*)(vu + i));
+    }
 }
 
 static int ffn_check(const char* what, int dtype, int M, int K, int F, int act) {
@@ -400,6 +493,8 @@ static int ffn_check(const char* what, int dtype, int M, int K, int F, int act) 
     NMPC_REQUIRE(M >= 0 && K >= 1 && F >= 1, "%s: bad sizes (%d rows, %d inputs, %d hidden units)", what, M, K, F);
     NMPC_REQUIRE(act >= NMPC_ACT_SILU && act <= NMPC_ACT_SIGMOID, "%s: activation %d", what, act);
     NMPC_REQUIRE(M < (1 << 22) && K < (1 << 21) && F < (1 << 21), "%s: at most 2^22 rows and 2^21 inputs and hidden units", what);
+    // a launch has fewer than 2^32 threads
+    NMPC_REQUIRE((M + 64ll) * (F / 2048 + 1) < (1 << 24), "%s: too many elements for one launch", what);
     return 0;
 }
 static unsigned long long round256(unsigned long long v) { return (v + 255) / 256 * 256; }
@@ -407,36 +502,47 @@ static unsigned long long round256(unsigned long long v) { return (v + 255) / 25
 constexpr int FEW_ROWS = 64;
 
 template <typename T>
-constexpr int ktile() { return 128 / (int)sizeof(T); }
+constexpr int ktile() { return 64 / (int)sizeof(T); }
 static int up_to(int v, int m) { return (v + m - 1) / m * m; }
 
-// whether a matrix can be read in whole 128-byte k-tiles as it is
+// whether a matrix with rows of K elements can be read in pieces of 16 bytes as it is; by k: in whole k-tiles
 template <typename T>
-static bool tiled(const void* p, long long ld, int K) {
-    return K % ktile<T>() == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * sizeof(T) % 16 == 0;
+static bool tiled(const void* p, long long ld, int K, bool by_k) {
+    return K % (by_k ? ktile<T>() : 16 / (int)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * sizeof(T) % 16 == 0;
 }
 
-// tile size and splits of a product: 256 x 256 where that gives the 256 CUs a tile each, else 128 x 128 (two workgroups a CU);
-// the contraction is split where tiles alone leave CUs idle, into parts of at least 8 k-tiles
+// Tile size and splits of a product: the choice of least estimated time.  A 256 x 256 tile has a CU for itself, two 128 x 128 tiles share
+// one; a k-tile of the large one takes 1.06 us in 16 bits and 4.0 us in fp32 (measured at 16384 x 2048 x 4096), of the small one a
+// quarter of it and a sixth more, less well used where a CU has one alone.  Every round of tiles pays for filling and draining; a split
+// contraction pays for writing and reading its partial products.
 struct Shape {
     bool large;
     int splits;
 };
+template <typename T>
 static Shape product_shape(int M, int N, int ktiles, bool may_split) {
-    const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256), small = (long long)((M + 127) / 128) * ((N + 127) / 128);
-    Shape s = {big >= 192, 1};
-    if (!s.large && may_split && small < 256) {
-        long long k = (512 + small - 1) / small;
-        if (k > ktiles / 8) k = ktiles / 8;
-        s.splits = k > 16 ? 16 : k < 1 ? 1 : (int)k;
+    const double ktime = sizeof(T) == 2 ? 1.06 : 4.0, fill = 4.0;
+    Shape best = {false, 1};
+    double least = 1e30;
+    for (int large = 0; large < 2; ++large) {
+        const int b = large ? 256 : 128;
+        const double tiles = (double)((M + b - 1) / b) * ((N + b - 1) / b);
+        for (int splits = 1; splits <= (may_split ? 16 : 1) && splits * 8 <= ktiles + 7; ++splits) {
+            const double n = tiles * splits, depth = (ktiles + splits - 1) / splits;
+            double t;
+            if (large) t = ceil(n / 256) * (depth * ktime + fill);
+            else t = n <= 256 ? depth * ktime * 0.25 * 1.5 + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
+            if (splits > 1) t += 6.0 + (double)splits * M * N * 8 / 4.5e6;
+            if (t < least) { least = t; best = {large != 0, splits}; }
+        }
     }
-    return s;
+    return best;
 }
 
-template <typename T, bool GATED>
+template <typename T, bool GATED, bool KA, bool KB>
 static int run_product(NtArgs g, hipStream_t st) {
     const int cols = GATED ? 2 * g.N : g.N;
-    const Shape shape = product_shape(g.M, cols, g.ktiles, !GATED && g.part);
+    const Shape shape = product_shape<T>(g.M, cols, g.ktiles, !GATED && g.part);
     g.splits = shape.splits;
     if (g.splits == 1) g.part = nullptr;
     const int bm = shape.large ? 256 : 128, bn = shape.large ? 256 : 128;
@@ -444,8 +550,8 @@ static int run_product(NtArgs g, hipStream_t st) {
     g.nt = (g.N + (GATED ? bn / 2 : bn) - 1) / (GATED ? bn / 2 : bn);
     const long long grid = (long long)g.mt * g.nt * g.splits;
     NMPC_REQUIRE(grid < (1 << 22), "gated_ffn: too many tiles for one launch");
-    if (shape.large) gemm_nt_kernel<T, 2, 4, 4, GATED><<<(unsigned)grid, 512, 0, st>>>(g);
-    else gemm_nt_kernel<T, 2, 2, 2, GATED><<<(unsigned)grid, 256, 0, st>>>(g);
+    if (shape.large) gemm_kernel<T, 2, 4, 4, GATED, KA, KB><<<(unsigned)grid, 512, 0, st>>>(g);
+    else gemm_kernel<T, 2, 2, 2, GATED, KA, KB><<<(unsigned)grid, 256, 0, st>>>(g);
     if (g.splits > 1) {
         const long long blocks = ((long long)g.M * g.N + 255) / 256;
         gemm_join_kernel<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(g);
@@ -459,79 +565,74 @@ static unsigned pad_grid(long long total) {
     return (unsigned)(blocks < 8192 ? blocks : 8192);
 }
 
-// The workspace of a call: copies of operands that cannot be read in k-tiles as they are, and the gradient's intermediates.
+// The workspace of a call: copies of operands that cannot be read in pieces as they are, and the gradient's intermediates.
 struct FfnSpace {
-    unsigned long long bytes, x, wg, wu, rows, cols, wt, xt, part;
+    unsigned long long bytes, x, wg, wu, rows, part;
+    int Kp;                            // row length of the copies
     template <typename T>
     static FfnSpace plan(int M, int K, int F, bool backward, bool copy) {
         FfnSpace s = {};
         const unsigned long long e = sizeof(T);
-        const int kt = ktile<T>(), Kp = up_to(K, kt), Fp = up_to(F, kt), Mp = up_to(M, kt);
+        const int kt = ktile<T>(), Fp = up_to(F, kt), Mp = up_to(M, kt);
         auto take = [&](unsigned long long bytes) { const unsigned long long at = s.bytes; s.bytes += round256(bytes); return at; };
-        if (!backward) {
-            if (M > FEW_ROWS && (copy || K % kt)) {
-                s.x = take(e * M * Kp);
-                s.wg = take(e * F * Kp);
-                s.wu = take(e * F * Kp);
-            }
-            return s;
+        s.Kp = up_to(K, backward ? 16 / (int)e : kt);
+        if ((backward || M > FEW_ROWS) && (copy || K != s.Kp)) {
+            s.x = take(e * M * s.Kp);
+            s.wg = take(e * F * s.Kp);
+            s.wu = take(e * F * s.Kp);
         }
-        s.rows = take(e * M * 2 * Fp);
-        s.cols = take(e * 2 * F * Mp);
-        s.wt = take(e * K * 2 * Fp);
-        s.xt = take(e * K * Mp);
-        const Shape a = product_shape(M, K, 2 * Fp / kt, true), b = product_shape(2 * F, K, Mp / kt, true);
-        const unsigned long long pa = a.splits > 1 ? 4ull * a.splits * M * K : 0, pb = b.splits > 1 ? 4ull * b.splits * 2 * F * K : 0;
+        if (!backward) return s;
+        s.rows = take(e * Mp * 2 * Fp);
+        const Shape a = product_shape<T>(M, K, 2 * Fp / kt, true), b = product_shape<T>(2 * Fp, K, Mp / kt, true);
+        const unsigned long long pa = a.splits > 1 ? 4ull * a.splits * M * K : 0, pb = b.splits > 1 ? 4ull * b.splits * 2 * Fp * K : 0;
         s.part = take(pa > pb ? pa : pb);
         return s;
     }
 };
+
+// the operands of a product as they are, or their copies in the workspace
 template <typename T>
-static bool needs_copy(int M, int K, const void* x, long long x_ld, const void* wg, const void* wu, long long w_ld) {
-    return M > FEW_ROWS && !(tiled<T>(x, x_ld, K) && tiled<T>(wg, w_ld, K) && tiled<T>(wu, w_ld, K));
+static int lay_out(const FfnSpace& sp, bool by_k, int M, int K, int F, const void*& x, long long& x_ld, const void*& wg, const void*& wu, long long& w_ld,
+                   char* ws, hipStream_t st) {
+    if (tiled<T>(x, x_ld, K, by_k) && tiled<T>(wg, w_ld, K, by_k) && tiled<T>(wu, w_ld, K, by_k)) return 0;
+    const int Kp = sp.Kp;
+    pad_kernel<T><<<pad_grid((long long)M * Kp), 256, 0, st>>>((const T*)x, x_ld, M, K, (T*)(ws + sp.x), Kp);
+    pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wg, w_ld, F, K, (T*)(ws + sp.wg), Kp);
+    pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wu, w_ld, F, K, (T*)(ws + sp.wu), Kp);
+    NMPC_HIP_CHECK(hipGetLastError());
+    x = ws + sp.x; wg = ws + sp.wg; wu = ws + sp.wu;
+    x_ld = w_ld = Kp;
+    return 0;
 }
 
 template <typename T>
 static int run_forward(int M, int K, int F, const void* x, long long x_ld, const void* wg, const void* wu, long long w_ld, int act, void* h,
                        float* pre, char* ws, unsigned long long ws_bytes, hipStream_t st) {
-    const bool copy = needs_copy<T>(M, K, x, x_ld, wg, wu, w_ld);
+    const bool copy = !(tiled<T>(x, x_ld, K, true) && tiled<T>(wg, w_ld, K, true) && tiled<T>(wu, w_ld, K, true));
     const FfnSpace sp = FfnSpace::plan<T>(M, K, F, false, copy);
     NMPC_REQUIRE(sp.bytes == 0 || (ws && ws_bytes >= sp.bytes), "nmpc_gated_ffn: workspace of %llu bytes, %llu needed", ws_bytes, sp.bytes);
     if (M <= FEW_ROWS) {
         constexpr int E = 16 / sizeof(T);
         FewArgs g = {x, wg, wu, x_ld, w_ld, M, K, F, act, h, pre};
         const bool al = K % E == 0 && vec_ok<T>(x, x_ld, 0, E) && vec_ok<T>(wg, w_ld, 0, E) && vec_ok<T>(wu, w_ld, 0, E);
-        const int blocks = (F + 15) / 16;
+        const int blocks = (F + 15) / 16, mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
         int waves = 4;                 // enough waves to keep the memory busy: about 2048 on the chip
-        while (waves < 16 && blocks * waves < 2048) waves *= 2;
-        const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+        while (waves < (mb == 4 ? 4 : 16) && blocks * waves < 2048) waves *= 2;
         const unsigned shared = waves * 2 * mb * 64 * 16;
-#define FEW(MB_)                                                                                                        \
+#define NMPC_FEW(MB_)                                                                                                   \
     if (al) gated_few_kernel<T, MB_, true><<<blocks, waves * 64, shared, st>>>(g);                                      \
     else gated_few_kernel<T, MB_, false><<<blocks, waves * 64, shared, st>>>(g);
-        if (mb == 1) { FEW(1) } else if (mb == 2) { FEW(2) } else {
-            while (waves > 4) waves /= 2;
-            const unsigned sh = waves * 2 * 4 * 64 * 16;
-            if (al) gated_few_kernel<T, 4, true><<<blocks, waves * 64, sh, st>>>(g);
-            else gated_few_kernel<T, 4, false><<<blocks, waves * 64, sh, st>>>(g);
-        }
-#undef FEW
+        if (mb == 1) { NMPC_FEW(1) } else if (mb == 2) { NMPC_FEW(2) } else { NMPC_FEW(4) }
+#undef NMPC_FEW
         NMPC_HIP_CHECK(hipGetLastError());
         return 0;
     }
+    if (lay_out<T>(sp, true, M, K, F, x, x_ld, wg, wu, w_ld, ws, st)) return 1;
     NtArgs g = {};
-    g.M = M; g.N = F; g.act = act; g.out = h; g.pre = pre; g.cut = M;
-    const int Kp = up_to(K, ktile<T>());
-    g.ktiles = Kp / ktile<T>();
-    if (copy) {
-        pad_kernel<T><<<pad_grid((long long)M * Kp), 256, 0, st>>>((const T*)x, x_ld, M, K, (T*)(ws + sp.x), Kp);
-        pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wg, w_ld, F, K, (T*)(ws + sp.wg), Kp);
-        pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wu, w_ld, F, K, (T*)(ws + sp.wu), Kp);
-        x = ws + sp.x; wg = ws + sp.wg; wu = ws + sp.wu;
-        x_ld = w_ld = Kp;
-    }
+    g.M = M; g.N = F; g.act = act; g.out = h; g.pre = pre;
+    g.ktiles = sp.Kp / ktile<T>();
     g.A = x; g.a_ld = x_ld; g.B = wg; g.B1 = wu; g.b_ld = w_ld;
-    return run_product<T, true>(g, st);
+    return run_product<T, true, true, true>(g, st);
 }
 
 template <typename T>
@@ -544,24 +645,27 @@ static int run_backward(int M, int K, int F, const void* x, long long x_ld, cons
         NMPC_HIP_CHECK(hipGetLastError());
         return 0;
     }
-    const FfnSpace sp = FfnSpace::plan<T>(M, K, F, true, false);
+    const bool copy = !(tiled<T>(x, x_ld, K, false) && tiled<T>(wg, w_ld, K, false) && tiled<T>(wu, w_ld, K, false));
+    const FfnSpace sp = FfnSpace::plan<T>(M, K, F, true, copy);
     NMPC_REQUIRE(ws && ws_bytes >= sp.bytes, "nmpc_gated_ffn_bwd: workspace of %llu bytes, %llu needed", ws_bytes, sp.bytes);
+    if (lay_out<T>(sp, false, M, K, F, x, x_ld, wg, wu, w_ld, ws, st)) return 1;
     const int kt = ktile<T>(), Fp = up_to(F, kt), Mp = up_to(M, kt);
-    T *rows = (T*)(ws + sp.rows), *cols = (T*)(ws + sp.cols), *wt = (T*)(ws + sp.wt), *xt = (T*)(ws + sp.xt);
-    const int mb = (Mp + 63) / 64, kb = (K + 63) / 64, fb = (Fp + 63) / 64;
-    gate_slope_kernel<T><<<dim3(mb, fb), 256, 0, st>>>(M, F, Mp, Fp, act, pre, (const T*)dh, dh_ld, rows, cols);
-    transpose_kernel<T><<<dim3(fb, kb), 256, 0, st>>>((const T*)wg, w_ld, F, K, wt, 2 * Fp, Fp);
-    transpose_kernel<T><<<dim3(fb, kb), 256, 0, st>>>((const T*)wu, w_ld, F, K, wt + Fp, 2 * Fp, Fp);
-    transpose_kernel<T><<<dim3(mb, kb), 256, 0, st>>>((const T*)x, x_ld, M, K, xt, Mp, Mp);
-    NtArgs g = {};
-    g.A = rows; g.a_ld = 2 * Fp; g.B = wt; g.b_ld = 2 * Fp;
-    g.M = M; g.N = K; g.ktiles = 2 * Fp / kt;
-    g.out = dx; g.cut = M; g.part = (float*)(ws + sp.part);
-    if (run_product<T, false>(g, st)) return 1;
-    g.A = cols; g.a_ld = Mp; g.B = xt; g.b_ld = Mp;
-    g.M = 2 * F; g.ktiles = Mp / kt;
-    g.out = dwg; g.out1 = dwu; g.cut = F;
-    return run_product<T, false>(g, st);
+    T* rows = (T*)(ws + sp.rows);
+    constexpr int E = 16 / sizeof(T);
+    const unsigned grid = (unsigned)Mp * (unsigned)((Fp / 8 + 255) / 256);
+    if (F % 8 == 0 && vec_ok<float>(pre, 0, 0, 4) && vec_ok<T>(dh, dh_ld, 0, E))
+        gate_slope_kernel<T, true><<<grid, 256, 0, st>>>(M, F, Mp, Fp, act, pre, (const T*)dh, dh_ld, rows);
+    else gate_slope_kernel<T, false><<<grid, 256, 0, st>>>(M, F, Mp, Fp, act, pre, (const T*)dh, dh_ld, rows);
+    NtArgs g = {};                     // dx = [dG dU] [Wg; Wu]
+    g.A = rows; g.a_ld = 2 * Fp; g.B = wg; g.B1 = wu; g.b_ld = w_ld;
+    g.M = M; g.N = K; g.ktiles = 2 * Fp / kt; g.kcut = Fp; g.b_kmax = F;
+    g.out = dx; g.cut = g.rows = M; g.part = (float*)(ws + sp.part);
+    if (run_product<T, false, true, false>(g, st)) return 1;
+    g = NtArgs{};                      // [dWg; dWu] = [dG dU]' x
+    g.A = rows; g.a_ld = 2 * Fp; g.a_kmax = Mp; g.B = x; g.b_ld = x_ld; g.kcut = Mp; g.b_kmax = M;
+    g.M = 2 * Fp; g.N = K; g.ktiles = Mp / kt;
+    g.out = dwg; g.out1 = dwu; g.cut = Fp; g.rows = F; g.part = (float*)(ws + sp.part);
+    return run_product<T, false, false, false>(g, st);
 }
 
 }  // namespace nmpc

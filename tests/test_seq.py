@@ -141,7 +141,7 @@ def test_scan_abi(tmp_path):
     assert L.nmpc_lpv_scan(None, None) != 0
     at, hold = args(nb=0)
     assert L.nmpc_lpv_scan(at, None) == 0 and L.nmpc_lpv_scan_step(at, None) == 0
-    assert L.nmpc_lpv_scan_saved_bytes(2, 33, 8, 5) == 2 * 2 * 8 * 8 * 4
+    assert L.nmpc_lpv_scan_saved_bytes(2, 33, 8, 5) == 2 * 3 * 8 * 8 * 4          # a state of 8 padded values before every 16th step
 
 
 def test_oracle_ffn_gradient_against_differences():

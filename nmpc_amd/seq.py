@@ -17,68 +17,93 @@ from ._lib import NmpcError, lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "tanh": 3, "sigmoid": 4}
+_Tensor = torch.Tensor
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+# The checks below run on every call of a kernel that takes a few microseconds: they test first and build a message only
+# where they refuse.
 
 
-def _need(ok, what, text, *args):
-    if not ok:
-        raise NmpcError("%s: %s" % (what, text % args if args else text))
+def _fail(what, text, *args):
+    raise NmpcError("%s: %s" % (what, text % args if args else text))
+
+
+def _got(t):
+    return list(t.shape) if isinstance(t, _Tensor) else type(t).__name__
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(dev, what, fn, *args):
-    """fn(*args, current stream of dev) with dev current; an error becomes NmpcError."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _call(i, what, fn, *args):
+    """fn(*args, current stream of GPU i) with that GPU current; an error becomes NmpcError."""
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, what)
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _on_gpu(what, x, *others):
-    """All tensors on x's GPU (checked last, after the shapes)."""
-    _lib.require_gpu()
-    _need(x.is_cuda, what, "tensors must be on the GPU, got %s", x.device)
+    """The number of the GPU that holds x and all others (checked last, after the shapes)."""
+    i = x.get_device()
+    if i < 0 or not x.is_cuda:
+        _lib.require_gpu()
+        _fail(what, "tensors must be on the GPU, got %s", x.device)
     for t in others:
-        _need(t is None or t.device == x.device, what, "tensors on different devices: %s and %s", x.device, getattr(t, "device", None))
+        if t is not None and t.get_device() != i:
+            _fail(what, "tensors on different devices: %s and %s", x.device, t.device)
+    return i
 
 
 def _samples(what, name, t, shape, dtype):
     """A sample tensor of this shape and type with contiguous channels (a copy only where they are not)."""
-    _need(torch.is_tensor(t) and tuple(t.shape) == tuple(shape), what, "%s must be %s, got %s", name, list(shape),
-          list(t.shape) if torch.is_tensor(t) else type(t).__name__)
-    _need(t.dtype == dtype, what, "%s is %s, the samples are %s", name, t.dtype, dtype)
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    if not isinstance(t, _Tensor) or t.shape != shape:
+        _fail(what, "%s must be %s, got %s", name, list(shape), _got(t))
+    if t.dtype is not dtype:
+        _fail(what, "%s is %s, the samples are %s", name, t.dtype, dtype)
+    return t if t.stride(-1) == 1 or shape[-1] == 1 else t.detach().contiguous()
 
 
 def _param(what, name, t, shape):
     """A parameter as contiguous fp32."""
-    _need(torch.is_tensor(t) and tuple(t.shape) == tuple(shape), what, "%s must be %s, got %s", name, list(shape),
-          list(t.shape) if torch.is_tensor(t) else type(t).__name__)
-    _need(t.is_floating_point(), what, "%s is %s, expected floating point", name, t.dtype)
-    t = t.detach()
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+    if not isinstance(t, _Tensor) or t.shape != shape:
+        _fail(what, "%s must be %s, got %s", name, list(shape), _got(t))
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
+    if not t.is_floating_point():
+        _fail(what, "%s is %s, expected floating point", name, t.dtype)
+    return t.detach().to(torch.float32).contiguous()
 
 
 def _lengths(what, t, nb):
     if t is None:
         return None
-    _need(torch.is_tensor(t) and t.dim() == 1 and t.shape[0] == nb, what, "lengths must be [%d]", nb)
-    _need(not t.is_floating_point() and not t.is_complex() and t.dtype != torch.bool, what, "lengths are %s, expected integers", t.dtype)
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if not isinstance(t, _Tensor) or t.shape != (nb,):
+        _fail(what, "lengths must be [%d], got %s", nb, _got(t))
+    if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+        _fail(what, "lengths are %s, expected integers", t.dtype)
+    if t.dtype is torch.int32 and t.is_contiguous():
+        return t
+    if t.element_size() > 4:                                   # values past int32 would wrap around: those above any length are one
+        t = t.clamp(-1, 2 ** 31 - 1)
+    return t.to(torch.int32).contiguous()
 
 
 def _records(what, *tensors):
     """Does this call have to be recorded by autograd?  Under graph capture it is refused: autograd's own bookkeeping of
     leaves that an eager graph still holds cannot be captured."""
-    if not torch.is_grad_enabled() or not any(torch.is_tensor(t) and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
         return False
-    _need(not (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()), what,
-          "autograd is not recorded under graph capture; capture the pair %s_fwd / %s_bwd (or call under torch.no_grad())", what, what)
-    return True
+    for t in tensors:
+        if isinstance(t, _Tensor) and t.requires_grad:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                _fail(what, "autograd is not recorded under graph capture; capture the pair %s_fwd / %s_bwd (or call under torch.no_grad())", what, what)
+            return True
+    return False
 
 
 class Saved:
@@ -91,7 +116,8 @@ class Saved:
 
 
 def _saved(what, saved):
-    _need(isinstance(saved, Saved) and saved.what == what, what + "_bwd", "expects what %s_fwd returned last", what)
+    if not isinstance(saved, Saved) or saved.what != what:
+        _fail(what + "_bwd", "expects what %s_fwd returned last", what)
     return saved.tensors, saved.values
 
 
@@ -114,37 +140,41 @@ class _Recorded(torch.autograd.Function):
 
 
 # ---- causal convolution ---------------------------------------------------------------------------------------------
-def _conv_args(what, u, w, bias, act, start, lengths, steps=True):
-    _need(torch.is_tensor(u) and u.dim() == (3 if steps else 2), what, "u must be %s", "[batch, steps, channels]" if steps else "[batch, channels]")
-    _need(u.dtype in _DTYPES, what, "samples are %s, expected float32, bfloat16 or float16", u.dtype)
-    _need(torch.is_tensor(w) and w.dim() == 2 and 1 <= w.shape[1] <= 8, what, "w must be [channels, taps] with 1..8 taps")
-    _need(act in (None, "none", "silu"), what, "activation %r (None or 'silu')", act)
-    nb, d, taps = u.shape[0], u.shape[-1], w.shape[1]
-    _need(d >= 1, what, "no channels")
-    w = _param(what, "w", w, (d, taps))
+def _conv_args(what, u, w, bias, act, steps):
+    if not isinstance(u, _Tensor) or u.dim() != (3 if steps else 2):
+        _fail(what, "u must be %s, got %s", "[batch, steps, channels]" if steps else "[batch, channels]", _got(u))
+    if u.dtype not in _DTYPES:
+        _fail(what, "samples are %s, expected float32, bfloat16 or float16", u.dtype)
+    if not isinstance(w, _Tensor) or w.dim() != 2 or not 1 <= w.shape[1] <= 8:
+        _fail(what, "w must be [channels, taps] with 1..8 taps, got %s", _got(w))
+    if act not in (None, "none", "silu"):
+        _fail(what, "activation %r (None or 'silu')", act)
+    d = u.shape[-1]
+    if d < 1:
+        _fail(what, "no channels")
+    w = _param(what, "w", w, (d, w.shape[1]))
     bias = None if bias is None else _param(what, "bias", bias, (d,))
-    if start is not None:
-        _need(steps or not torch.is_tensor(start) or start.is_contiguous(), what, "window must be a contiguous tensor: it is moved on in place")
-        start = _samples(what, "start" if steps else "window", start, (nb, taps - 1, d), u.dtype).contiguous()
-    u = u if u.stride(-1) == 1 or d == 1 else u.contiguous()
-    return u, w, bias, start, _lengths(what, lengths, nb)
+    return u if u.stride(-1) == 1 or d == 1 else u.detach().contiguous(), w, bias
 
 
 def _conv_fwd(what, u, w, bias, act, start, lengths, want_window):
-    u, w, bias, start, lengths = _conv_args(what, u, w, bias, act, start, lengths)
-    _on_gpu(what, u, w, bias, start, lengths)
+    u, w, bias = _conv_args(what, u, w, bias, act, True)
     nb, steps, d = u.shape
+    taps = w.shape[1]
+    if start is not None:
+        start = _samples(what, "start", start, (nb, taps - 1, d), u.dtype).contiguous()
+    lengths = _lengths(what, lengths, nb)
+    i = _on_gpu(what, u, w, bias, start, lengths)
     y = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
-    window = torch.empty((nb, w.shape[1] - 1, d), dtype=u.dtype, device=u.device) if want_window else None
-    _call(u.device, what, lib().nmpc_causal_conv, _DTYPES[u.dtype], nb, steps, d, w.shape[1], _p(u), u.stride(0), u.stride(1), _p(w),
-          _p(bias), _ACTS[act], _p(start), _p(lengths), _p(y), _p(window))
+    window = torch.empty((nb, taps - 1, d), dtype=u.dtype, device=u.device) if want_window else None
+    _call(i, what, lib().nmpc_causal_conv, _DTYPES[u.dtype], nb, steps, d, taps, u.data_ptr(), u.stride(0), u.stride(1), w.data_ptr(),
+          _p(bias), _ACTS[act], _p(start), _p(lengths), y.data_ptr(), _p(window))
     return y, window, (u, w, bias, start, lengths)
 
 
 def causal_conv_fwd(u, w, bias=None, act=None, start=None, lengths=None):
     """causal_conv that keeps what its gradient needs: (y, window, saved)."""
-    with torch.no_grad():
-        y, window, tensors = _conv_fwd("causal_conv_fwd", u, w, bias, act, start, lengths, True)
+    y, window, tensors = _conv_fwd("causal_conv_fwd", u, w, bias, act, start, lengths, True)
     return y, window, Saved("causal_conv", tensors, (act,))
 
 
@@ -157,16 +187,16 @@ def causal_conv_bwd(saved, dy, dwindow=None):
     taps = w.shape[1]
     dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
     dwindow = None if dwindow is None else _samples(what, "dwindow", dwindow, (nb, taps - 1, d), u.dtype).contiguous()
-    _on_gpu(what, u, dy, dwindow)
+    i = _on_gpu(what, u, dy, dwindow)
     du = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
     dw = torch.empty_like(w)
     dbias = None if bias is None else torch.empty_like(bias)
     dstart = None if start is None else torch.empty_like(start)
     size = lib().nmpc_causal_conv_workspace_bytes(nb, steps, d, taps)
     work = torch.empty(size, dtype=torch.uint8, device=u.device)
-    _call(u.device, what, lib().nmpc_causal_conv_bwd, _DTYPES[u.dtype], nb, steps, d, taps, _p(u), u.stride(0), u.stride(1), _p(w),
-          _p(bias), _ACTS[act], _p(start), _p(lengths), _p(dy), dy.stride(0), dy.stride(1), _p(dwindow), _p(du), _p(dw), _p(dbias),
-          _p(dstart), _p(work), size)
+    _call(i, what, lib().nmpc_causal_conv_bwd, _DTYPES[u.dtype], nb, steps, d, taps, u.data_ptr(), u.stride(0), u.stride(1), w.data_ptr(),
+          _p(bias), _ACTS[act], _p(start), _p(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1), _p(dwindow), du.data_ptr(),
+          dw.data_ptr(), _p(dbias), _p(dstart), work.data_ptr(), size)
     return {"du": du, "dw": dw, "dbias": dbias, "dstart": dstart}
 
 
@@ -178,8 +208,7 @@ def causal_conv(u, w, bias=None, act=None, start=None, lengths=None, return_stat
     [batch, taps-1, channels] of the last samples: the start of what follows, and causal_conv_step's state."""
     what = "causal_conv"
     if not _records(what, u, w, bias, start):
-        with torch.no_grad():
-            y, window, _ = _conv_fwd(what, u, w, bias, act, start, lengths, return_state)
+        y, window, _ = _conv_fwd(what, u, w, bias, act, start, lengths, return_state)
         return (y, window) if return_state else y
 
     def fwd():
@@ -197,67 +226,74 @@ def causal_conv_step(window, u, w, bias=None, act=None):
     """One sample u [batch, channels] of every sequence: returns y [batch, channels] and moves window [batch, taps-1,
     channels] (contiguous) on by one row in place."""
     what = "causal_conv_step"
-    _need(not _records(what, window, u, w, bias), what, "works in place and has no gradient; use causal_conv")
-    u, w, bias, window, _ = _conv_args(what, u, w, bias, act, window, None, steps=False)
-    _need(window is not None, what, "needs a window")
-    _on_gpu(what, u, w, bias, window)
-    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-    _call(u.device, what, lib().nmpc_causal_conv_step, _DTYPES[u.dtype], u.shape[0], u.shape[1], w.shape[1], _p(window), _p(u),
-          u.stride(0), _p(w), _p(bias), _ACTS[act], _p(y))
+    if _records(what, window, u, w, bias):
+        _fail(what, "works in place and has no gradient; use causal_conv")
+    u, w, bias = _conv_args(what, u, w, bias, act, False)
+    nb, d = u.shape
+    taps = w.shape[1]
+    if isinstance(window, _Tensor) and not window.is_contiguous():
+        _fail(what, "window must be a contiguous tensor: it is moved on in place")
+    _samples(what, "window", window, (nb, taps - 1, d), u.dtype)
+    i = _on_gpu(what, u, w, bias, window)
+    y = torch.empty((nb, d), dtype=u.dtype, device=u.device)
+    _call(i, what, lib().nmpc_causal_conv_step, _DTYPES[u.dtype], nb, d, taps, window.data_ptr(), u.data_ptr(), u.stride(0),
+          w.data_ptr(), _p(bias), _ACTS[act], y.data_ptr())
     return y
 
 
 # ---- selective LPV scan ---------------------------------------------------------------------------------------------
-def _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, steps=True):
-    lead = 2 if steps else 1
-    _need(torch.is_tensor(u) and u.dim() == lead + 1, what, "u must be %s", "[batch, steps, channels]" if steps else "[batch, channels]")
-    _need(u.dtype in _DTYPES, what, "samples are %s, expected float32, bfloat16 or float16", u.dtype)
-    d = u.shape[-1]
-    _need(torch.is_tensor(A) and A.dim() == 2 and A.shape[0] == d and 1 <= A.shape[1] <= 64, what, "A must be [channels, states] with 1..64 states")
+def _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, lead):
+    """The checked inputs; lead: leading dimensions of the samples (batch, steps)."""
+    if not isinstance(u, _Tensor) or u.dim() != lead + 1:
+        _fail(what, "u must be %s, got %s", "[batch, steps, channels]" if lead == 2 else "[batch, channels]", _got(u))
+    dtype, shape = u.dtype, u.shape
+    if dtype not in _DTYPES:
+        _fail(what, "samples are %s, expected float32, bfloat16 or float16", dtype)
+    d = shape[-1]
+    if not isinstance(A, _Tensor) or A.dim() != 2 or A.shape[0] != d or not 1 <= A.shape[1] <= 64:
+        _fail(what, "A must be [channels, states] with 1..64 states, got %s", _got(A))
     n = A.shape[1]
-    _need(torch.is_tensor(B) and B.dim() == lead + 2 and B.shape[:lead] == u.shape[:lead] and B.shape[-1] == n, what,
-          "B must be %s", list(u.shape[:lead]) + ["groups", n])
+    if not isinstance(B, _Tensor) or B.dim() != lead + 2 or B.shape[:lead] != shape[:lead] or B.shape[-1] != n:
+        _fail(what, "B must be %s, got %s", list(shape[:lead]) + ["groups", n], _got(B))
     groups = B.shape[-2]
-    _need(d >= 1 and groups >= 1 and d % groups == 0, what, "%d groups do not divide %d channels", groups, d)
-    u = u if u.stride(-1) == 1 or d == 1 else u.contiguous()
-    dt = _samples(what, "dt", dt, u.shape, u.dtype)
-    z = None if z is None else _samples(what, "z", z, u.shape, u.dtype)
-
-    def shared(name, t):
-        t = _samples(what, name, t, tuple(u.shape[:lead]) + (groups, n), u.dtype)
-        return t if groups == 1 or t.stride(-2) == n else t.contiguous()
-    return (u, dt, _param(what, "A", A, (d, n)), shared("B", B), shared("C", C), None if D is None else _param(what, "D", D, (d,)), z,
+    if d < 1 or groups < 1 or d % groups:
+        _fail(what, "%d groups do not divide %d channels", groups, d)
+    u = u if u.stride(-1) == 1 or d == 1 else u.detach().contiguous()
+    dt = _samples(what, "dt", dt, shape, dtype)
+    if z is not None:
+        z = _samples(what, "z", z, shape, dtype)
+    C = _samples(what, "C", C, B.shape, dtype)
+    B = _samples(what, "B", B, B.shape, dtype)
+    if groups > 1:
+        B = B if B.stride(-2) == n else B.detach().contiguous()
+        C = C if C.stride(-2) == n else C.detach().contiguous()
+    return (u, dt, _param(what, "A", A, (d, n)), B, C, None if D is None else _param(what, "D", D, (d,)), z,
             None if dt_bias is None else _param(what, "dt_bias", dt_bias, (d,)))
 
 
 def _scan_struct(u, dt, A, B, C, D, z, dt_bias, softplus):
     """The argument struct with the inputs filled in; unused strides of single steps stay zero."""
-    s = _lib.ScanArgs()
-    s.struct_size, s.dtype, s.nb, s.D, s.softplus = ctypes.sizeof(_lib.ScanArgs), _DTYPES[u.dtype], u.shape[0], u.shape[-1], int(bool(softplus))
-    s.N, s.G = A.shape[1], B.shape[-2]
-    s.u, s.dt, s.A, s.B, s.C = u.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr()
-    s.u_bs, s.dt_bs, s.B_bs, s.C_bs = u.stride(0), dt.stride(0), B.stride(0), C.stride(0)
-    if D is not None:
-        s.D_skip = D.data_ptr()
-    if dt_bias is not None:
-        s.dt_bias = dt_bias.data_ptr()
-    if z is not None:
-        s.z, s.z_bs = z.data_ptr(), z.stride(0)
+    s = _lib.ScanArgs(_SCAN_SIZE, _DTYPES[u.dtype], u.shape[0], 1, u.shape[-1], A.shape[1], B.shape[-2], 1 if softplus else 0,
+                      u.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), _p(z), u.stride(0), 0, dt.stride(0), 0, B.stride(0), 0,
+                      C.stride(0), 0, 0 if z is None else z.stride(0), 0, A.data_ptr(), _p(D), _p(dt_bias))
     if u.dim() == 3:
         s.L, s.u_ts, s.dt_ts, s.B_ts, s.C_ts = u.shape[1], u.stride(1), dt.stride(1), B.stride(1), C.stride(1)
         if z is not None:
             s.z_ts = z.stride(1)
-    else:
-        s.L = 1
     return s
+
+
+_SCAN_SIZE = ctypes.sizeof(_lib.ScanArgs)
 
 
 def _states(what, name, t, nb, A):
     if t is None:
         return None
-    _need(torch.is_tensor(t) and tuple(t.shape) == (nb,) + tuple(A.shape), what, "%s must be %s", name, [nb] + list(A.shape))
-    _need(t.dtype == torch.float32, what, "%s is %s, states are float32", name, t.dtype)
-    return t.contiguous()
+    if not isinstance(t, _Tensor) or t.shape != (nb,) + A.shape:
+        _fail(what, "%s must be %s, got %s", name, [nb] + list(A.shape), _got(t))
+    if t.dtype is not torch.float32:
+        _fail(what, "%s is %s, states are float32", name, t.dtype)
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _scan_work(s, dev, backward):
@@ -270,10 +306,10 @@ def _scan_work(s, dev, backward):
 
 
 def _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, want_state, want_saved):
-    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias)
+    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, 2)
     nb, steps, d = u.shape
     start, lengths = _states(what, "start", start, nb, A), _lengths(what, lengths, nb)
-    _on_gpu(what, *tensors, start, lengths)
+    i = _on_gpu(what, *tensors, start, lengths)
     s = _scan_struct(*tensors, softplus)
     s.start, s.lengths = _p(start), _p(lengths)
     y = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
@@ -283,15 +319,14 @@ def _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, wan
         saved = torch.empty(lib().nmpc_lpv_scan_saved_bytes(nb, steps, d, A.shape[1]), dtype=torch.uint8, device=u.device)
     s.y, s.last, s.saved = y.data_ptr(), _p(last), _p(saved)
     work = _scan_work(s, u.device, 0)  # noqa: F841  (held until the launch)
-    _call(u.device, what, lib().nmpc_lpv_scan, ctypes.addressof(s))
+    _call(i, what, lib().nmpc_lpv_scan, ctypes.addressof(s))
     return y, last, tensors + (start, lengths, saved)
 
 
 def lpv_scan_fwd(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, start=None, lengths=None):
     """lpv_scan that keeps what its gradient needs: (y, last, saved).  Besides the inputs that is the state before every
-    32nd step."""
-    with torch.no_grad():
-        y, last, tensors = _scan_fwd("lpv_scan_fwd", u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, True, True)
+    16th step."""
+    y, last, tensors = _scan_fwd("lpv_scan_fwd", u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, True, True)
     return y, last, Saved("lpv_scan", tensors, (bool(softplus),))
 
 
@@ -303,7 +338,7 @@ def lpv_scan_bwd(saved, dy, dlast=None):
     (u, dt, A, B, C, D, z, dt_bias, start, lengths, kept), (softplus,) = _saved("lpv_scan", saved)
     dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
     dlast = _states(what, "dlast", dlast, u.shape[0], A)
-    _on_gpu(what, u, dy, dlast)
+    i = _on_gpu(what, u, dy, dlast)
     s = _scan_struct(u, dt, A, B, C, D, z, dt_bias, softplus)
     s.lengths, s.saved, s.dy, s.dy_bs, s.dy_ts, s.dlast = _p(lengths), _p(kept), dy.data_ptr(), dy.stride(0), dy.stride(1), _p(dlast)
     like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
@@ -312,7 +347,7 @@ def lpv_scan_bwd(saved, dy, dlast=None):
     for name, t in g.items():
         setattr(s, name, _p(t))
     work = _scan_work(s, u.device, 1)  # noqa: F841  (held until the launch)
-    _call(u.device, what, lib().nmpc_lpv_scan_bwd, ctypes.addressof(s))
+    _call(i, what, lib().nmpc_lpv_scan_bwd, ctypes.addressof(s))
     return g
 
 
@@ -326,8 +361,7 @@ def lpv_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, start=
     zeros).  Returns y, with return_state also the state after the last step, lpv_scan_step's state."""
     what = "lpv_scan"
     if not _records(what, u, dt, A, B, C, D, z, dt_bias, start):
-        with torch.no_grad():
-            y, last, _ = _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, return_state, False)
+        y, last, _ = _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, return_state, False)
         return (y, last) if return_state else y
 
     def fwd():
@@ -346,32 +380,37 @@ def lpv_scan_step(state, u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=
     """One sample of every sequence: u, dt, z [batch, channels], B, C [batch, groups, states].  Returns y [batch, channels];
     state [batch, channels, states] (fp32, contiguous) moves on by one step in place."""
     what = "lpv_scan_step"
-    _need(not _records(what, state, u, dt, A, B, C, D, z, dt_bias), what, "works in place and has no gradient; use lpv_scan")
-    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, steps=False)
-    _need(torch.is_tensor(state) and state.is_contiguous(), what, "state must be a contiguous tensor: it is moved on in place")
-    state = _states(what, "state", state, u.shape[0], A)
-    _on_gpu(what, *tensors, state)
+    if _records(what, state, u, dt, A, B, C, D, z, dt_bias):
+        _fail(what, "works in place and has no gradient; use lpv_scan")
+    u, dt, A, B, C, D, z, dt_bias = tensors = _scan_inputs(what, u, dt, A, B, C, D, z, dt_bias, 1)
+    if not isinstance(state, _Tensor) or not state.is_contiguous():
+        _fail(what, "state must be a contiguous tensor: it is moved on in place")
+    _states(what, "state", state, u.shape[0], A)
+    i = _on_gpu(what, *tensors, state)
     s = _scan_struct(*tensors, softplus)
     y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
     s.y, s.last = y.data_ptr(), state.data_ptr()
-    _call(u.device, what, lib().nmpc_lpv_scan_step, ctypes.addressof(s))
+    _call(i, what, lib().nmpc_lpv_scan_step, ctypes.addressof(s))
     return y
 
 
 # ---- gated feed-forward projections ---------------------------------------------------------------------------------
 def _ffn_args(what, x, w_gate, w_up, act):
-    _need(torch.is_tensor(x) and x.dim() >= 1, what, "x must be [..., inputs]")
-    _need(x.dtype in _DTYPES, what, "x is %s, expected float32, bfloat16 or float16", x.dtype)
-    k = x.shape[-1]
-    _need(torch.is_tensor(w_gate) and w_gate.dim() == 2 and w_gate.shape[1] == k and k >= 1 and w_gate.shape[0] >= 1, what,
-          "w_gate must be [hidden, %d]", k)
-    _need(act in ("silu", "gelu", "tanh", "sigmoid"), what, "activation %r (silu, gelu, tanh or sigmoid)", act)
-    w_gate = _samples(what, "w_gate", w_gate, w_gate.shape, x.dtype)
-    w_up = _samples(what, "w_up", w_up, w_gate.shape, x.dtype)
+    if not isinstance(x, _Tensor) or x.dim() < 1:
+        _fail(what, "x must be [..., inputs], got %s", _got(x))
+    dtype, k = x.dtype, x.shape[-1]
+    if dtype not in _DTYPES:
+        _fail(what, "x is %s, expected float32, bfloat16 or float16", dtype)
+    if not isinstance(w_gate, _Tensor) or w_gate.dim() != 2 or w_gate.shape[1] != k or k < 1 or w_gate.shape[0] < 1:
+        _fail(what, "w_gate must be [hidden, %d], got %s", k, _got(w_gate))
+    if act not in ("silu", "gelu", "tanh", "sigmoid"):
+        _fail(what, "activation %r (silu, gelu, tanh or sigmoid)", act)
+    w_up = _samples(what, "w_up", w_up, w_gate.shape, dtype)
+    w_gate = _samples(what, "w_gate", w_gate, w_gate.shape, dtype)
     if w_gate.stride(0) != w_up.stride(0):
-        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
-    rows = x.reshape(-1, k)
-    return rows if rows.stride(-1) == 1 or k == 1 else rows.contiguous(), w_gate, w_up
+        w_gate, w_up = w_gate.detach().contiguous(), w_up.detach().contiguous()
+    rows = x if x.dim() == 2 else x.detach().reshape(-1, k)
+    return rows if rows.stride(-1) == 1 or k == 1 else rows.detach().contiguous(), w_gate, w_up
 
 
 def _ffn_work(x, w_gate, w_up, backward):
@@ -382,20 +421,19 @@ def _ffn_work(x, w_gate, w_up, backward):
 
 def _ffn_fwd(what, x, w_gate, w_up, act, want_saved):
     rows, w_gate, w_up = _ffn_args(what, x, w_gate, w_up, act)
-    _on_gpu(what, rows, w_gate, w_up)
+    i = _on_gpu(what, rows, w_gate, w_up)
     (m, k), f = rows.shape, w_gate.shape[0]
     h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
     pre = torch.empty((2, m, f), dtype=torch.float32, device=x.device) if want_saved else None
     work, size = _ffn_work(rows, w_gate, w_up, 0)
-    _call(x.device, what, lib().nmpc_gated_ffn, _DTYPES[x.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate), w_gate.stride(0),
-          _p(w_up), w_up.stride(0), _ACTS[act], _p(h), _p(pre), _p(work), size)
+    _call(i, what, lib().nmpc_gated_ffn, _DTYPES[x.dtype], m, k, f, rows.data_ptr(), rows.stride(0), w_gate.data_ptr(), w_gate.stride(0),
+          w_up.data_ptr(), w_up.stride(0), _ACTS[act], h.data_ptr(), _p(pre), _p(work), size)
     return h, (rows, w_gate, w_up, pre)
 
 
 def gated_ffn_fwd(x, w_gate, w_up, act="silu"):
     """gated_ffn that keeps what its gradient needs: (h, saved).  Besides the inputs that is both projections in fp32."""
-    with torch.no_grad():
-        h, tensors = _ffn_fwd("gated_ffn_fwd", x, w_gate, w_up, act, True)
+    h, tensors = _ffn_fwd("gated_ffn_fwd", x, w_gate, w_up, act, True)
     return h, Saved("gated_ffn", tensors, (act, tuple(x.shape)))
 
 
@@ -405,12 +443,13 @@ def gated_ffn_bwd(saved, dh):
     (rows, w_gate, w_up, pre), (act, shape) = _saved("gated_ffn", saved)
     (m, k), f = rows.shape, w_gate.shape[0]
     dh = _samples(what, "dh", dh, shape[:-1] + (f,), rows.dtype).reshape(m, f)
-    _on_gpu(what, rows, dh)
+    i = _on_gpu(what, rows, dh)
     dx = torch.empty(shape, dtype=rows.dtype, device=rows.device)
     dwg, dwu = (torch.empty((f, k), dtype=rows.dtype, device=rows.device) for _ in range(2))
     work, size = _ffn_work(rows, w_gate, w_up, 1)
-    _call(rows.device, what, lib().nmpc_gated_ffn_bwd, _DTYPES[rows.dtype], m, k, f, _p(rows), rows.stride(0), _p(w_gate),
-          w_gate.stride(0), _p(w_up), w_up.stride(0), _ACTS[act], _p(pre), _p(dh), dh.stride(0), _p(dx), _p(dwg), _p(dwu), _p(work), size)
+    _call(i, what, lib().nmpc_gated_ffn_bwd, _DTYPES[rows.dtype], m, k, f, rows.data_ptr(), rows.stride(0), w_gate.data_ptr(),
+          w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), _ACTS[act], pre.data_ptr(), dh.data_ptr(), dh.stride(0), dx.data_ptr(),
+          dwg.data_ptr(), dwu.data_ptr(), _p(work), size)
     return dx, dwg, dwu
 
 
@@ -421,8 +460,7 @@ def gated_ffn(x, w_gate, w_up, act="silu"):
     few (tokens of running sequences) and many rows (prompts, training) take kernels of their own."""
     what = "gated_ffn"
     if not _records(what, x, w_gate, w_up):
-        with torch.no_grad():
-            return _ffn_fwd(what, x, w_gate, w_up, act, False)[0]
+        return _ffn_fwd(what, x, w_gate, w_up, act, False)[0]
 
     def fwd():
         h, saved = gated_ffn_fwd(x, w_gate, w_up, act)

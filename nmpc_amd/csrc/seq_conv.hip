@@ -2,15 +2,21 @@
 //   line = [start (W-1 rows); u],   s[t,c] = bias[c] + sum_j w[c,j] line[t+j,c],   y = act(s).
 // Gradients, with ds = dy act'(s):
 //   dline[k,c] = sum_j w[c,j] ds[k-j,c]  (+ dwindow where row k is one of the last W-1),   dw[c,j] = sum ds[t,c] line[t+j,c].
-// All of it is bound by memory: one read of u and one write of y (backward: u, dy in, du out).  A thread owns 16 bytes of
-// neighbouring channels and a run of time steps; the W-1 rows behind the run are read again by the next one, everything
-// else of the filter stays in registers.  Arithmetic and sums are fp32.
+// All of it is bound by memory: one read of u and one write of y (backward: u, dy in, du out).  A thread owns a few neighbouring
+// channels and a run of 16 steps; the W-1 rows before the run (backward: behind it) are read again by the neighbouring run, mostly
+// from the L2 cache, and everything else of the filter stays in registers.  Arithmetic and sums are fp32.
+// Channels of a thread, measured at bf16 4 x 2048 x 4096, W = 4: forward 8 bytes 28 us (4.8 TB/s; 16 bytes 37 us: half the waves),
+// backward 4 bytes 61 us (3.3 TB/s; 8 bytes 76 us and 16 bytes 115 us: the unrolled run then takes 216 and over 256 registers).
+// Runs of 32 steps need 185 registers instead of 121 in the backward pass: 82 us.
+#include <type_traits>
+
 #include "seq_common.h"
 
 namespace nmpc {
 
 constexpr int CONV_MAX_W = 8;
 constexpr int CONV_TR = 16;          // steps of one thread
+constexpr int CONV_GROUP = 4;        // steps whose loads are in flight together
 
 struct ConvArgs {
     int nb, L, D, silu, nch, ncv;
@@ -66,21 +72,34 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
             for (int i = 0; i < VEC; ++i) win[j][i] = (float)r.v[i];
         }
     }
-#pragma unroll 4
-    for (int t = t0; t < tv; ++t) {
-        const Vec<T, VEC> r = load_vec<T, VEC>(ub + t * a.u_ts);
-        Vec<T, VEC> o;
+    // all loads of a group of steps before its first store (the compiler cannot know that y is not u)
+    auto group = [&](int tg, auto whole) {
+        Vec<T, VEC> rows[CONV_GROUP];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            win[W - 1][i] = (float)r.v[i];
-            float s = bias[i];
+        for (int k = 0; k < CONV_GROUP; ++k)
+            if (whole.value || tg + k < tv) rows[k] = load_vec<T, VEC>(ub + (tg + k) * a.u_ts);
 #pragma unroll
-            for (int j = 0; j < W; ++j) s += w[j][i] * win[j][i];
-            o.v[i] = (T)(a.silu ? s * sigmoid(s) : s);
+        for (int k = 0; k < CONV_GROUP; ++k) {
+            if (!whole.value && tg + k >= tv) break;
+            Vec<T, VEC> o;
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
+            for (int i = 0; i < VEC; ++i) {
+                win[W - 1][i] = (float)rows[k].v[i];
+                float s = bias[i];
+#pragma unroll
+                for (int j = 0; j < W; ++j) s += w[j][i] * win[j][i];
+                o.v[i] = (T)(a.silu ? s * sigmoid(s) : s);
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
+            }
+            store_vec(yb + (long long)(tg + k) * a.D, o);
         }
-        store_vec(yb + (long long)t * a.D, o);
+    };
+    if (tv == t0 + CONV_TR) {
+#pragma unroll
+        for (int k = 0; k < CONV_TR; k += CONV_GROUP) group(t0 + k, std::true_type{});
+    } else {
+        for (int tg = t0; tg < tv; tg += CONV_GROUP) group(tg, std::false_type{});
     }
     Vec<T, VEC> zero;
 #pragma unroll
@@ -95,9 +114,8 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
 
 // ds of step t and the step's row of u; `win` holds the W-1 rows before it and is shifted
 template <typename T, int W, int VEC>
-__device__ __forceinline__ void conv_slope(const ConvArgs& a, const T* ub, const T* gb, int t, const float (&w)[W][VEC],
+__device__ __forceinline__ void conv_slope(int silu, const Vec<T, VEC>& r, const Vec<T, VEC>& g, const float (&w)[W][VEC],
                                            const float (&bias)[VEC], float (&win)[W][VEC], float (&ds)[VEC]) {
-    const Vec<T, VEC> r = load_vec<T, VEC>(ub + t * a.u_ts), g = load_vec<T, VEC>(gb + t * a.dy_ts);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         win[W - 1][i] = (float)r.v[i];
@@ -105,7 +123,7 @@ __device__ __forceinline__ void conv_slope(const ConvArgs& a, const T* ub, const
 #pragma unroll
         for (int j = 0; j < W; ++j) s += w[j][i] * win[j][i];
         float k = (float)g.v[i];
-        if (a.silu) {
+        if (silu) {
             const float p = sigmoid(s);
             k *= p * (1.f + s * (1.f - p));
         }
@@ -154,10 +172,13 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
             }
         }
         // row k of the line's gradient is complete once ds of steps k-W+1 .. k is known
-        for (int t = t0; t < tv + W - 1; ++t) {
-            if (t < len) {
-                conv_slope<T, W, VEC>(a, ub, gb, t, w, bias, win, ds[W - 1]);
-                if (t < tv) {
+        const int tl = min(tv + W - 1, len);           // steps that are read
+        // step k of the run; whole: all W - 1 steps behind the run are inside the sequence, so that only k decides
+        auto step = [&](int k, const Vec<T, VEC>& ru, const Vec<T, VEC>& rg, auto whole) {
+            const int t = t0 + k;
+            if (whole.value || t < tl) {
+                conv_slope<T, W, VEC>(a.silu, ru, rg, w, bias, win, ds[W - 1]);
+                if (whole.value ? k < CONV_TR : t < tv) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
 #pragma unroll
@@ -173,23 +194,52 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) ds[W - 1][i] = 0.f;
             }
-            const int s = t - (W - 1);                 // u[s] is row t of the line; it feeds steps s .. t
-            if (s >= t0 && s < tv) {
+            if (k >= W - 1) {                          // u[t - W + 1] is row t of the line; it feeds steps t - W + 1 .. t
                 Vec<T, VEC> o, e;
-                if (eb && t >= len) e = load_vec<T, VEC>(eb + (long long)(t - len) * a.D);
+                const bool end = !whole.value && eb && t >= len;
+                if (end) e = load_vec<T, VEC>(eb + (long long)(t - len) * a.D);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    float v = eb && t >= len ? (float)e.v[i] : 0.f;
+                    float v = end ? (float)e.v[i] : 0.f;
 #pragma unroll
                     for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * ds[j][i];
                     o.v[i] = (T)v;
                 }
-                store_vec(db + (long long)s * a.D, o);
+                store_vec(db + (long long)(t - (W - 1)) * a.D, o);
             }
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) ds[j][i] = ds[j + 1][i];
+        };
+        if (tv == t0 + CONV_TR && tl == tv + W - 1) {
+            constexpr int STEPS = CONV_TR + W - 1;
+            Vec<T, VEC> ru[2][CONV_GROUP], rg[2][CONV_GROUP];      // the next group's rows are loaded while this one's are used
+            auto fetch = [&](int g) {
+#pragma unroll
+                for (int k = 0; k < CONV_GROUP; ++k)
+                    if (g * CONV_GROUP + k < STEPS) {
+                        ru[g & 1][k] = load_vec<T, VEC>(ub + (t0 + g * CONV_GROUP + k) * a.u_ts);
+                        rg[g & 1][k] = load_vec<T, VEC>(gb + (t0 + g * CONV_GROUP + k) * a.dy_ts);
+                    }
+            };
+            fetch(0);
+#pragma unroll
+            for (int g = 0; g * CONV_GROUP < STEPS; ++g) {
+                if ((g + 1) * CONV_GROUP < STEPS) fetch(g + 1);
+#pragma unroll
+                for (int k = 0; k < CONV_GROUP; ++k)
+                    if (g * CONV_GROUP + k < STEPS) step(g * CONV_GROUP + k, ru[g & 1][k], rg[g & 1][k], std::true_type{});
+            }
+        } else {
+            for (int t = t0; t < tv + W - 1; ++t) {
+                Vec<T, VEC> ru, rg;
+                if (t < tl) {
+                    ru = load_vec<T, VEC>(ub + t * a.u_ts);
+                    rg = load_vec<T, VEC>(gb + t * a.dy_ts);
+                }
+                step(t - t0, ru, rg, std::false_type{});
+            }
         }
         Vec<T, VEC> zero;
 #pragma unroll
@@ -207,7 +257,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
             for (int t = 0; t < W - 1; ++t)
                 if (t < len) {
-                    conv_slope<T, W, VEC>(a, ub, gb, t, w, bias, win, ds[0]);
+                    conv_slope<T, W, VEC>(a.silu, load_vec<T, VEC>(ub + t * a.u_ts), load_vec<T, VEC>(gb + t * a.dy_ts), w, bias, win, ds[0]);
 #pragma unroll
                     for (int k = t; k < W - 1; ++k)
 #pragma unroll
@@ -322,7 +372,7 @@ extern "C" int nmpc_causal_conv(int dtype, int nb, int L, int D, int W, const vo
     a.u = u; a.u_bs = u_bs; a.u_ts = u_ts; a.w = w; a.bias = bias; a.start = start; a.lengths = lengths;
     a.y = y; a.window = W > 1 ? window : nullptr;
     NMPC_DTYPE_SWITCH(dtype, {
-        constexpr int V = 16 / sizeof(T_);
+        constexpr int V = 8 / sizeof(T_);
         const bool vec = D % V == 0 && vec_ok<T_>(u, u_bs, u_ts, V) && vec_ok<T_>(start, 0, 0, V) && vec_ok<T_>(y, 0, 0, V) &&
                          vec_ok<T_>(window, 0, 0, V);
         a.ncv = vec ? D / V : D;
@@ -360,7 +410,7 @@ extern "C" int nmpc_causal_conv_bwd(int dtype, int nb, int L, int D, int W, cons
     a.nrb = 0;
     if (nb > 0 && (L > 0 || a.dstart)) {
         NMPC_DTYPE_SWITCH(dtype, {
-            constexpr int V = 16 / sizeof(T_);
+            constexpr int V = 4 / sizeof(T_);
             const bool vec = D % V == 0 && vec_ok<T_>(u, u_bs, u_ts, V) && vec_ok<T_>(start, 0, 0, V) && vec_ok<T_>(dy, dy_bs, dy_ts, V) &&
                              vec_ok<T_>(dwindow, 0, 0, V) && vec_ok<T_>(du, 0, 0, V) && vec_ok<T_>(dstart, 0, 0, V);
             a.ncv = vec ? D / V : D;
@@ -390,7 +440,7 @@ extern "C" int nmpc_causal_conv_step(int dtype, int nb, int D, int W, void* wind
     a.nb = nb; a.L = 1; a.D = D; a.silu = act == NMPC_ACT_SILU;
     a.u = u; a.u_bs = u_bs; a.w = w; a.bias = bias; a.y = y; a.window = window;
     NMPC_DTYPE_SWITCH(dtype, {
-        constexpr int V = 16 / sizeof(T_);
+        constexpr int V = 8 / sizeof(T_);
         const bool vec = D % V == 0 && vec_ok<T_>(u, u_bs, 0, V) && vec_ok<T_>(y, 0, 0, V) && vec_ok<T_>(window, 0, 0, V);
         a.ncv = vec ? D / V : D;
         const unsigned grid = (unsigned)(((long long)nb * a.ncv + 255) / 256);

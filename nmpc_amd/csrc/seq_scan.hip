@@ -701,40 +701,63 @@ __global__ __launch_bounds__(256) void scan_reduce_bc_kernel(ScanDev s, int NP) 
     }
 }
 
-// One step of every sequence; the state a.last is read and replaced.
-template <typename T, int P>
+// One step of every sequence; the state a.last is read and replaced: 8 N bytes a channel, which is the time.  FOUR: N is a multiple
+// of 4 and a lane's four states, decays, B and C are one access each.
+template <typename T, int P, bool FOUR>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanDev s) {
     const nmpc_scan_args& a = s.a;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, bc = id / P;
-    const int q = (int)(id % P), b = (int)(bc / a.D), ch = (int)(bc % a.D);
+    const unsigned id = blockIdx.x * 256u + threadIdx.x, bc = id / P;
+    const int q = (int)(id % P), b = (int)(bc / (unsigned)a.D), ch = (int)(bc % (unsigned)a.D);
     if (b >= a.nb) return;                            // the P lanes of a channel leave together
-    const int g = ch / s.per;
-    float A[4], x[4];
-    load_A<P>(s, ch, true, q, A);
-    float* state = a.last + bc * a.N;
-    load_states(state, a.N, q, x);
+    const int n0 = 4 * q;
+    const long long g = (long long)(ch / s.per) * a.N + n0;
+    const T* Bp = (const T*)a.B + b * a.B_bs + g;
+    const T* Cp = (const T*)a.C + b * a.C_bs + g;
+    const float* Ap = a.A + (long long)ch * a.N + n0;
+    float* state = a.last + (long long)bc * a.N + n0;
+    float A[4], x[4], B[4], C[4];
+    if (FOUR) {
+        if (n0 < a.N) {
+            load_four(Ap, A);
+            load_four(state, x);
+            const Vec<T, 4> vb = load_vec<T, 4>(Bp), vc = load_vec<T, 4>(Cp);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { B[i] = (float)vb.v[i]; C[i] = (float)vc.v[i]; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A[i] = x[i] = B[i] = C[i] = 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = n0 + i < a.N;
+            A[i] = in ? Ap[i] : 0.f;
+            x[i] = in ? state[i] : 0.f;
+            B[i] = in ? (float)Bp[i] : 0.f;
+            C[i] = in ? (float)Cp[i] : 0.f;
+        }
+    }
     const float uu = (float)((const T*)a.u)[b * a.u_bs + ch];
     float d = (float)((const T*)a.dt)[b * a.dt_bs + ch] + (a.dt_bias ? a.dt_bias[ch] : 0.f);
+    const float zz = a.z ? (float)((const T*)a.z)[b * a.z_bs + ch] : 0.f;
     if (a.softplus) d = softplus(d);
-    const T* Bp = (const T*)a.B + b * a.B_bs + (long long)g * a.N;
-    const T* Cp = (const T*)a.C + b * a.C_bs + (long long)g * a.N;
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int n = 4 * q + i;
-        if (n < a.N) {
-            x[i] = __builtin_amdgcn_exp2f(d * A[i]) * x[i] + (d * uu) * (float)Bp[n];
-            y += (float)Cp[n] * x[i];
-        }
+        x[i] = __builtin_amdgcn_exp2f(d * (A[i] * LOG2E)) * x[i] + (d * uu) * B[i];
+        y += C[i] * x[i];
     }
-    store_states(state, a.N, q, x);
+    if (FOUR) {
+        if (n0 < a.N) store_four(state, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n0 + i < a.N) state[i] = x[i];
+    }
     y = sum_lanes<P>(y);
     if (q == 0) {
         if (a.D_skip) y += a.D_skip[ch] * uu;
-        if (a.z) {
-            const float zz = (float)((const T*)a.z)[b * a.z_bs + ch];
-            y *= zz * sigmoid(zz);
-        }
+        if (a.z) y *= zz * sigmoid(zz);
         ((T*)a.y)[bc] = (T)y;
     }
 }
@@ -904,7 +927,10 @@ extern "C" int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream) {
     scan_plan(s);
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
-            scan_step_kernel<T_, P_><<<(unsigned)(((long long)a.nb * a.D * P_ + 255) / 256), 256, 0, (hipStream_t)stream>>>(s);
+            const unsigned grid = (unsigned)(((long long)a.nb * a.D * P_ + 255) / 256);
+            if (a.N % 4 == 0 && vec_ok<float>(a.A, 0, 0, 4) && vec_ok<float>(a.last, 0, 0, 4) && vec_ok<T_>(a.B, a.B_bs, 0, 4) && vec_ok<T_>(a.C, a.C_bs, 0, 4))
+                scan_step_kernel<T_, P_, true><<<grid, 256, 0, (hipStream_t)stream>>>(s);
+            else scan_step_kernel<T_, P_, false><<<grid, 256, 0, (hipStream_t)stream>>>(s);
         })
     })
     NMPC_HIP_CHECK(hipGetLastError());

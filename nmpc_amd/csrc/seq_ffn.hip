@@ -329,8 +329,9 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(NtArgs g) {
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// Up to 64 rows of x: the weights are read once, which is the time.  A workgroup owns 16 hidden units of both projections and
-// shares the contraction among its waves; their partial products are joined through LDS in wave order.
+// Few rows of x, or few products altogether.  A workgroup owns 16 hidden units of both projections and 16 MB rows (blockIdx.y) and
+// shares the contraction among its waves, whose partial products are joined through LDS in wave order.  Up to 64 rows the weights are
+// read once, which is the time; operands go from memory to the matrix cores without LDS, any alignment.
 struct FewArgs {
     const void *x, *wg, *wu;
     long long x_ld, w_ld;
@@ -363,19 +364,35 @@ struct Mma16<float> {
     }
 };
 
-// 16 bytes of a row from element k on, zero past its end
+// 16 bytes of a row from element k on, zero past its end.  Unaligned rows are read as the dwords that hold the piece (each holds a valid
+// element, so that none lies outside the matrix's memory) and shifted; only a row's last piece goes element by element.
+typedef unsigned u32x4_dword __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ uint4 row_piece(const T* row, int k, int K, bool ok) {
     constexpr int E = 16 / sizeof(T);
+    uint4 v = make_uint4(0, 0, 0, 0);
     if constexpr (ALIGNED) {           // whole pieces: K is a multiple of E
-        if (ok && k < K) return *reinterpret_cast<const uint4*>(row + k);
-        return make_uint4(0, 0, 0, 0);
-    } else {
-        Vec<T, E> v;
+        if (ok && k < K) v = *reinterpret_cast<const uint4*>(row + k);
+    } else if (ok && k + E <= K) {
+        const unsigned long long a = (unsigned long long)(row + k);
+        const unsigned* p = (const unsigned*)(a & ~3ull);
+        const u32x4_dword d = *(const u32x4_dword*)p;
+        if constexpr (sizeof(T) == 4) {
+            v = make_uint4(d.x, d.y, d.z, d.w);
+        } else {
+            const unsigned shift = (unsigned)(a & 2) * 8, last = p[shift ? 4 : 3];
+            v.x = __builtin_amdgcn_alignbit(d.y, d.x, shift);
+            v.y = __builtin_amdgcn_alignbit(d.z, d.y, shift);
+            v.z = __builtin_amdgcn_alignbit(d.w, d.z, shift);
+            v.w = __builtin_amdgcn_alignbit(last, d.w, shift);
+        }
+    } else if (ok && k < K) {
+        Vec<T, E> t;
 #pragma unroll
-        for (int i = 0; i < E; ++i) v.v[i] = ok && k + i < K ? row[k + i] : (T)0.f;
-        return __builtin_bit_cast(uint4, v);
+        for (int i = 0; i < E; ++i) t.v[i] = k + i < K ? row[k + i] : (T)0.f;
+        v = __builtin_bit_cast(uint4, t);
     }
+    return v;
 }
 
 template <typename T, int MB, bool ALIGNED>
@@ -383,7 +400,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(FewArgs g) {
     constexpr int E = 16 / sizeof(T), BK = 4 * E, UN = MB == 1 ? 4 : 2;
     extern __shared__ f32x4 red[];     // [waves][2 MB][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int r = lane & 15, f = blockIdx.x * 16 + r;
+    const int r = lane & 15, f = blockIdx.x * 16 + r, m0 = blockIdx.y * 16 * MB;
     const bool okf = f < g.F;
     const T* wg = (const T*)g.wg + (long long)(okf ? f : 0) * g.w_ld;
     const T* wu = (const T*)g.wu + (long long)(okf ? f : 0) * g.w_ld;
@@ -391,7 +408,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(FewArgs g) {
     f32x4 acc[2][MB] = {};
     const T* xr[MB];
 #pragma unroll
-    for (int b = 0; b < MB; ++b) xr[b] = (const T*)g.x + (long long)min(b * 16 + r, g.M - 1) * g.x_ld;
+    for (int b = 0; b < MB; ++b) xr[b] = (const T*)g.x + (long long)min(m0 + b * 16 + r, g.M - 1) * g.x_ld;
     for (int s = s0; s < s1; s += UN) {
         uint4 a0[UN], a1[UN], bx[UN][MB];
 #pragma unroll
@@ -400,7 +417,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(FewArgs g) {
             a0[i] = row_piece<T, ALIGNED>(wg, k, g.K, okf);
             a1[i] = row_piece<T, ALIGNED>(wu, k, g.K, okf);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) bx[i][b] = row_piece<T, ALIGNED>(xr[b], k, g.K, b * 16 + r < g.M);
+            for (int b = 0; b < MB; ++b) bx[i][b] = row_piece<T, ALIGNED>(xr[b], k, g.K, m0 + b * 16 + r < g.M);
         }
 #pragma unroll
         for (int i = 0; i < UN; ++i)
@@ -422,7 +439,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(FewArgs g) {
             gate += red[w * 2 * MB * 64 + e];
             up += red[(w * 2 * MB + MB) * 64 + e];
         }
-        const int m = (e >> 6) * 16 + (e & 15);
+        const int m = m0 + (e >> 6) * 16 + (e & 15);
         if (m >= g.M) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -436,13 +453,20 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(FewArgs g) {
 }
 
 // ---- operands laid out for the products ------------------------------------------------------------------------------
-// dst[row][0 .. ld): src row, zero from `cols` on
+// up to three matrices: dst[row][0 .. ld): src row, zero from `cols` on
+struct PadArgs {
+    const void* src[3];
+    long long s_ld[3];
+    void* dst[3];
+    int rows[3], cols, ld;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void pad_kernel(const T* src, long long s_ld, int rows, int cols, T* dst, int ld) {
-    const long long total = (long long)rows * ld;
+__global__ __launch_bounds__(256) void pad_kernel(PadArgs p) {
+    const int k = blockIdx.y;
+    const long long total = (long long)p.rows[k] * p.ld;
     for (long long o = (long long)blockIdx.x * 256 + threadIdx.x; o < total; o += 256ll * gridDim.x) {
-        const int c = (int)(o % ld);
-        dst[o] = c < cols ? src[(o / ld) * s_ld + c] : (T)0.f;
+        const int c = (int)(o % p.ld);
+        ((T*)p.dst[k])[o] = c < p.cols ? ((const T*)p.src[k])[(o / p.ld) * p.s_ld[k] + c] : (T)0.f;
     }
 }
 
@@ -518,25 +542,57 @@ static bool tiled(const void* p, long long ld, int K, bool by_k) {
 struct Shape {
     bool large;
     int splits;
+    double us;
 };
 template <typename T>
 static Shape product_shape(int M, int N, int ktiles, bool may_split) {
     const double ktime = sizeof(T) == 2 ? 1.06 : 4.0, fill = 4.0;
-    Shape best = {false, 1};
-    double least = 1e30;
+    Shape best = {false, 1, 1e30};
     for (int large = 0; large < 2; ++large) {
         const int b = large ? 256 : 128;
         const double tiles = (double)((M + b - 1) / b) * ((N + b - 1) / b);
-        for (int splits = 1; splits <= (may_split ? 16 : 1) && splits * 8 <= ktiles + 7; ++splits) {
+        for (int splits = 1; splits <= (may_split ? 64 : 1) && (splits == 1 || splits * 4 <= ktiles); ++splits) {
             const double n = tiles * splits, depth = (ktiles + splits - 1) / splits;
             double t;
             if (large) t = ceil(n / 256) * (depth * ktime + fill);
-            else t = n <= 256 ? depth * ktime * 0.25 * 1.5 + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
+            else t = n <= 256 ? depth * ktime * 0.25 * (sizeof(T) == 2 ? 1.25 : 1.0) + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
             if (splits > 1) t += 6.0 + (double)splits * M * N * 8 / 4.5e6;
-            if (t < least) { least = t; best = {large != 0, splits}; }
+            if (t < best.us) best = {large != 0, splits, t};
         }
     }
     return best;
+}
+
+// How the kernel for few rows would run a forward pass: rows of a workgroup as many as leave every CU one (at most 64: the weights are
+// read once for them), and its estimated time.  A step of 64 bytes of k of 64 rows x 16 units takes 0.68 ns of the chip in 16 bits (the
+// rate of the cache lines its loads touch) and 1.03 ns in fp32 (its products), 1.0 and 1.2 ns on unaligned rows; measured at
+// 512 x 2048 x 2048 and 333 x 1001 x 2731.
+struct FewShape {
+    int mb, waves;
+    dim3 grid;
+    double us;
+};
+template <typename T>
+static FewShape few_shape(int M, int K, int F, bool aligned) {
+    FewShape s = {4, 4, dim3((F + 15) / 16, 1), 0.0};
+    auto rows = [&] { return (M + 16 * s.mb - 1) / (16 * s.mb); };
+    while (s.mb > 1 && (8 * s.mb >= M || (long long)s.grid.x * rows() < 256)) s.mb /= 2;
+    s.grid.y = rows();
+    const double blocks = (double)s.grid.x * s.grid.y;
+    while (s.waves < (s.mb == 4 ? 8 : 16) && blocks * s.waves < 2048) s.waves *= 2;
+    const double ns = sizeof(T) == 2 ? (aligned ? 0.68 : 1.0) : (aligned ? 1.03 : 1.2);
+    const double steps = blocks * ((K + ktile<T>() - 1) / ktile<T>()) * (sizeof(T) == 2 ? (2 + s.mb) / 6.0 : s.mb / 4.0);
+    s.us = 4.0 + steps * ns * 1e-3 * (blocks < 256 ? 256 / blocks : 1.0);
+    return s;
+}
+
+// Does it?  Up to 64 rows always; beyond, where its estimate is below that of the tiles, which leave most CUs idle when there are few of
+// them and need copies of unaligned operands.
+template <typename T>
+static bool serves_few(int M, int K, int F, bool aligned) {
+    if (M <= FEW_ROWS) return true;
+    if ((M + 15) / 16 > 65535) return false;
+    return few_shape<T>(M, K, F, aligned).us < product_shape<T>(M, 2 * F, (K + ktile<T>() - 1) / ktile<T>(), false).us + (aligned ? 0.0 : 6.0);
 }
 
 template <typename T, bool GATED, bool KA, bool KB>
@@ -576,7 +632,7 @@ struct FfnSpace {
         const int kt = ktile<T>(), Fp = up_to(F, kt), Mp = up_to(M, kt);
         auto take = [&](unsigned long long bytes) { const unsigned long long at = s.bytes; s.bytes += round256(bytes); return at; };
         s.Kp = up_to(K, backward ? 16 / (int)e : kt);
-        if ((backward || M > FEW_ROWS) && (copy || K != s.Kp)) {
+        if ((copy || K != s.Kp) && (backward || !serves_few<T>(M, K, F, false))) {
             s.x = take(e * M * s.Kp);
             s.wg = take(e * F * s.Kp);
             s.wu = take(e * F * s.Kp);
@@ -596,9 +652,8 @@ static int lay_out(const FfnSpace& sp, bool by_k, int M, int K, int F, const voi
                    char* ws, hipStream_t st) {
     if (tiled<T>(x, x_ld, K, by_k) && tiled<T>(wg, w_ld, K, by_k) && tiled<T>(wu, w_ld, K, by_k)) return 0;
     const int Kp = sp.Kp;
-    pad_kernel<T><<<pad_grid((long long)M * Kp), 256, 0, st>>>((const T*)x, x_ld, M, K, (T*)(ws + sp.x), Kp);
-    pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wg, w_ld, F, K, (T*)(ws + sp.wg), Kp);
-    pad_kernel<T><<<pad_grid((long long)F * Kp), 256, 0, st>>>((const T*)wu, w_ld, F, K, (T*)(ws + sp.wu), Kp);
+    const PadArgs p = {{x, wg, wu}, {x_ld, w_ld, w_ld}, {ws + sp.x, ws + sp.wg, ws + sp.wu}, {M, F, F}, K, Kp};
+    pad_kernel<T><<<dim3(pad_grid((long long)(M > F ? M : F) * Kp), 3), 256, 0, st>>>(p);
     NMPC_HIP_CHECK(hipGetLastError());
     x = ws + sp.x; wg = ws + sp.wg; wu = ws + sp.wu;
     x_ld = w_ld = Kp;
@@ -611,17 +666,17 @@ static int run_forward(int M, int K, int F, const void* x, long long x_ld, const
     const bool copy = !(tiled<T>(x, x_ld, K, true) && tiled<T>(wg, w_ld, K, true) && tiled<T>(wu, w_ld, K, true));
     const FfnSpace sp = FfnSpace::plan<T>(M, K, F, false, copy);
     NMPC_REQUIRE(sp.bytes == 0 || (ws && ws_bytes >= sp.bytes), "nmpc_gated_ffn: workspace of %llu bytes, %llu needed", ws_bytes, sp.bytes);
-    if (M <= FEW_ROWS) {
+    if (serves_few<T>(M, K, F, !copy)) {
         constexpr int E = 16 / sizeof(T);
         FewArgs g = {x, wg, wu, x_ld, w_ld, M, K, F, act, h, pre};
         const bool al = K % E == 0 && vec_ok<T>(x, x_ld, 0, E) && vec_ok<T>(wg, w_ld, 0, E) && vec_ok<T>(wu, w_ld, 0, E);
-        const int blocks = (F + 15) / 16, mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-        int waves = 4;                 // enough waves to keep the memory busy: about 2048 on the chip
-        while (waves < (mb == 4 ? 4 : 16) && blocks * waves < 2048) waves *= 2;
+        const FewShape fs = few_shape<T>(M, K, F, al);
+        const dim3 grid = fs.grid;
+        const int mb = fs.mb, waves = fs.waves;
         const unsigned shared = waves * 2 * mb * 64 * 16;
 #define NMPC_FEW(MB_)                                                                                                   \
-    if (al) gated_few_kernel<T, MB_, true><<<blocks, waves * 64, shared, st>>>(g);                                      \
-    else gated_few_kernel<T, MB_, false><<<blocks, waves * 64, shared, st>>>(g);
+    if (al) gated_few_kernel<T, MB_, true><<<grid, waves * 64, shared, st>>>(g);                                        \
+    else gated_few_kernel<T, MB_, false><<<grid, waves * 64, shared, st>>>(g);
         if (mb == 1) { NMPC_FEW(1) } else if (mb == 2) { NMPC_FEW(2) } else { NMPC_FEW(4) }
 #undef NMPC_FEW
         NMPC_HIP_CHECK(hipGetLastError());
@@ -640,8 +695,8 @@ static int run_backward(int M, int K, int F, const void* x, long long x_ld, cons
                         const float* pre, const void* dh, long long dh_ld, void* dx, void* dwg, void* dwu, char* ws,
                         unsigned long long ws_bytes, hipStream_t st) {
     if (M == 0) {
-        pad_kernel<T><<<pad_grid((long long)F * K), 256, 0, st>>>(nullptr, 0, F, 0, (T*)dwg, K);
-        pad_kernel<T><<<pad_grid((long long)F * K), 256, 0, st>>>(nullptr, 0, F, 0, (T*)dwu, K);
+        const PadArgs p = {{}, {}, {dwg, dwu}, {F, F}, 0, K};      // nothing but zeros
+        pad_kernel<T><<<dim3(pad_grid((long long)F * K), 2), 256, 0, st>>>(p);
         NMPC_HIP_CHECK(hipGetLastError());
         return 0;
     }

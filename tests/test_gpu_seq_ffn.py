@@ -21,7 +21,7 @@ def _inputs(seed, m, k, f, dtype):
 def _bounds(x, wg, wu, dh, name):
     """Absolute error that fp32 arithmetic and the operands' rounding may cause, per output."""
     half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
-    x, wg, wu, dh = f64(x), f64(wg), f64(wu), f64(dh)
+    x, wg, wu, dh = (t.detach().double() for t in (x, wg, wu, dh))
     k, f = x.shape[1], wg.shape[0]
     gate, up = x @ wg.T, x @ wu.T
     eg, eu = (2 * k * U32 * (x.abs() @ w.abs().T) for w in (wg, wu))
@@ -69,6 +69,25 @@ def test_forward_and_gradients(m, k, f, dtype, name):
     assert torch.equal(nmpc_amd.gated_ffn(x.cuda(), wg.cuda(), wu.cuda(), name), got["h"])
     again = _run(x, wg, wu, dh, name)
     assert all(torch.equal(got[key], again[key]) for key in got), "the same call gives the same bits"
+
+
+@pytest.mark.parametrize("m,k,f,dtype,name", [
+    (700, 1032, 1500, "bf16", "silu"),        # tiles of 128 x 128, k tail
+    (2200, 160, 4104, "f16", "gelu"),         # tiles of 256 x 256, ragged in both directions
+    (640, 320, 1800, "f32", "tanh"),
+    (2049, 96, 4100, "bf16", "sigmoid"),      # odd rows, hidden units not a multiple of 8
+    (150, 72, 9000, "f32", "silu"),           # contraction of the gradients split
+])
+def test_many_tiles(m, k, f, dtype, name):
+    """The same at sizes of many tiles; the definition is evaluated in fp64 on the GPU."""
+    x, wg, wu, dh = (t.cuda() for t in _inputs(m, m, k, f, dtype))
+    lx, lg, lu = (t.double().requires_grad_() for t in (x, wg, wu))
+    ho = oracle.gated_ffn(lx, lg, lu, name)
+    want = dict(zip(("dx", "dwg", "dwu"), torch.autograd.grad(ho, (lx, lg, lu), dh.double())), h=ho)
+    got = _run(x, wg, wu, dh, name)
+    bound = _bounds(x, wg, wu, dh, name)
+    for key in ("h", "dx", "dwg", "dwu"):
+        assert_close(got[key], want[key], 1 / U32, bound[key].cpu(), key)
 
 
 def test_no_rows():

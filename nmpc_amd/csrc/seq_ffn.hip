@@ -462,12 +462,21 @@ struct PadArgs {
 };
 template <typename T>
 __global__ __launch_bounds__(256) void pad_kernel(PadArgs p) {
+    constexpr int E = 16 / sizeof(T);
     const int k = blockIdx.y;
-    const long long total = (long long)p.rows[k] * p.ld;
+    const unsigned pieces = (unsigned)(p.ld / E);
+    const long long total = (long long)p.rows[k] * pieces;
     for (long long o = (long long)blockIdx.x * 256 + threadIdx.x; o < total; o += 256ll * gridDim.x) {
-        const int c = (int)(o % p.ld);
-        ((T*)p.dst[k])[o] = c < p.cols ? ((const T*)p.src[k])[(o / p.ld) * p.s_ld[k] + c] : (T)0.f;
+        const long long row = total < (1ll << 32) ? (unsigned)o / pieces : o / pieces;
+        const int c = (int)(o - row * pieces) * E;
+        *reinterpret_cast<uint4*>((T*)p.dst[k] + row * p.ld + c) = row_piece<T, false>((const T*)p.src[k] + row * p.s_ld[k], c, p.cols, true);
     }
+}
+
+// zeros
+template <typename T>
+__global__ __launch_bounds__(256) void zero_kernel(T* p, long long n) {
+    for (long long o = (long long)blockIdx.x * 256 + threadIdx.x; o < n; o += 256ll * gridDim.x) p[o] = (T)0.f;
 }
 
 // dG, dU from the saved projections: rows [Mp][2 Fp], dG then dU, zero past M and past F.  Bound by memory (2 e + 2 e + 8 + e bytes an
@@ -653,7 +662,7 @@ static int lay_out(const FfnSpace& sp, bool by_k, int M, int K, int F, const voi
     if (tiled<T>(x, x_ld, K, by_k) && tiled<T>(wg, w_ld, K, by_k) && tiled<T>(wu, w_ld, K, by_k)) return 0;
     const int Kp = sp.Kp;
     const PadArgs p = {{x, wg, wu}, {x_ld, w_ld, w_ld}, {ws + sp.x, ws + sp.wg, ws + sp.wu}, {M, F, F}, K, Kp};
-    pad_kernel<T><<<dim3(pad_grid((long long)(M > F ? M : F) * Kp), 3), 256, 0, st>>>(p);
+    pad_kernel<T><<<dim3(pad_grid((long long)(M > F ? M : F) * Kp * (long long)sizeof(T) / 16), 3), 256, 0, st>>>(p);
     NMPC_HIP_CHECK(hipGetLastError());
     x = ws + sp.x; wg = ws + sp.wg; wu = ws + sp.wu;
     x_ld = w_ld = Kp;
@@ -695,8 +704,8 @@ static int run_backward(int M, int K, int F, const void* x, long long x_ld, cons
                         const float* pre, const void* dh, long long dh_ld, void* dx, void* dwg, void* dwu, char* ws,
                         unsigned long long ws_bytes, hipStream_t st) {
     if (M == 0) {
-        const PadArgs p = {{}, {}, {dwg, dwu}, {F, F}, 0, K};      // nothing but zeros
-        pad_kernel<T><<<dim3(pad_grid((long long)F * K), 2), 256, 0, st>>>(p);
+        zero_kernel<T><<<pad_grid((long long)F * K), 256, 0, st>>>((T*)dwg, (long long)F * K);
+        zero_kernel<T><<<pad_grid((long long)F * K), 256, 0, st>>>((T*)dwu, (long long)F * K);
         NMPC_HIP_CHECK(hipGetLastError());
         return 0;
     }

@@ -669,22 +669,33 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_bwd_kernel(
     }
 }
 
-// Sums of the partial sums over sequences and chunks (dA, dD, the bias) and over channel blocks (dB, dC), in a fixed order.
+// Sums of the partial sums over sequences and chunks (dA, dD, the bias) and over channel blocks (dB, dC), in a fixed order: four
+// threads share a parameter's rows, each with four sums of its own, so that the loads of many rows are in flight.
 __global__ __launch_bounds__(256) void scan_reduce_params_kernel(ScanDev s, int NP) {
+    __shared__ float red[256];
     const nmpc_scan_args& a = s.a;
-    const long long rows = (long long)a.nb * s.nch, id = (long long)blockIdx.x * 256 + threadIdx.x, nA = (long long)a.D * NP;
-    if (id < nA) {
-        float v = 0.f;
-        for (long long r = 0; r < rows; ++r) v += s.pA[r * nA + id];
+    const long long rows = (long long)a.nb * s.nch, id = (long long)blockIdx.x * 64 + (threadIdx.x & 63), nA = (long long)a.D * NP;
+    const int sub = threadIdx.x >> 6;
+    const bool is_A = id < nA, is_b = !is_A && id < nA + 2 * a.D;
+    const float* p = is_A ? s.pA + id : s.pDb + (id - nA);
+    const long long step = is_A ? nA : 2 * a.D;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (is_A || is_b)
+        for (long long r = sub; r < rows; r += 16)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (r + 4 * k < rows) v[k] += p[(r + 4 * k) * step];
+    red[threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
+    __syncthreads();
+    if (sub) return;
+    const float sum = (red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
+    if (is_A) {
         const int n = (int)(id % NP);
-        if (n < a.N) a.dA[(id / NP) * a.N + n] = v;
-    } else if (id < nA + 2 * a.D) {
-        const int k = (int)((id - nA) / a.D), ch = (int)((id - nA) % a.D);
+        if (n < a.N) a.dA[(id / NP) * a.N + n] = sum;
+    } else if (is_b) {
+        const int k = (int)((id - nA) / a.D);
         float* out = k ? a.ddt_bias : a.dD;
-        if (!out) return;
-        float v = 0.f;
-        for (long long r = 0; r < rows; ++r) v += s.pDb[(r * 2 + k) * a.D + ch];
-        out[ch] = v;
+        if (out) out[(id - nA) % a.D] = sum;
     }
 }
 template <typename T>
@@ -772,13 +783,19 @@ static void scan_plan(ScanDev& s) {
     s.ntile = a.L > 0 ? (a.L + SCAN_T - 1) / SCAN_T : 0;
     s.nch = 1;
     s.tpc = s.ntile;
-    const long long base = (long long)a.nb * a.G * s.nblk;
-    const int target = 1024;           // workgroups: four a CU
+    // Workgroups of whole sequences alone fill the chip from about 512 on (two a CU).  With fewer the time axis is cut into chunks, at the
+    // price of a pass that summarises each chunk: 3.6 of 5.6 ps a channel and step at N = 16.  bf16, 16 states: 1 x 8192 x 2048 takes 1025 us
+    // whole, 172 us with 512 workgroups, 160 us with 1024 and 157 us with 2048; 4 x 2048 x 2048 262, 164, 150 and 140 us (1 x 2048 x 2048: 248,
+    // 55, 56 and 67 us); 8 x 2048 x 4096 (512 workgroups whole) 372 us whole, 540 us in chunks.  A tile takes 4 us one after the other, the
+    // summary 2.6 us a tile and 8 us in launches: short sequences stay whole.
+    const long long base = (long long)a.nb * a.G * s.nblk, target = 1024;
     if (base > 0 && base * 2 <= target && s.ntile > 1) {
         const long long want = (target + base - 1) / base;
-        const int n = want < s.ntile ? (int)want : s.ntile;
-        s.tpc = (s.ntile + n - 1) / n;
-        s.nch = (s.ntile + s.tpc - 1) / s.tpc;
+        const int n = want < s.ntile ? (int)want : s.ntile, tpc = (s.ntile + n - 1) / n;
+        if (tpc * 6.6 + 8 < s.ntile * 4.0) {
+            s.tpc = tpc;
+            s.nch = (s.ntile + tpc - 1) / tpc;
+        }
     }
 }
 
@@ -908,7 +925,7 @@ extern "C" int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream) {
                 if (pairs) scan_bwd_kernel<T_, P_, V_><<<grid, SCAN_THREADS, 0, st>>>(s);
                 else scan_bwd_kernel<T_, P_, 1><<<grid, SCAN_THREADS, 0, st>>>(s);
             }
-            scan_reduce_params_kernel<<<(unsigned)(((long long)a.D * (NP + 2) + 255) / 256), 256, 0, st>>>(s, NP);
+            scan_reduce_params_kernel<<<(unsigned)(((long long)a.D * (NP + 2) + 63) / 64), 256, 0, st>>>(s, NP);
             const long long nbc = (long long)a.nb * a.L * a.G * 2 * NP;
             if (nbc > 0) scan_reduce_bc_kernel<T_><<<(unsigned)std::min((nbc + 255) / 256, 1ll << 20), 256, 0, st>>>(s, NP);
         })

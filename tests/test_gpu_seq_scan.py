@@ -132,6 +132,26 @@ def test_long_records(nb, steps, d, n, dtype, lengths):
     _check(v, dy, dlast, True, lengths)
 
 
+def test_chunks_of_several_tiles():
+    """128 sequences of 17 tiles are cut into chunks of three tiles (the last of two), a sequence alone into chunks of one."""
+    v, dy, dlast = _inputs(2, 128, 520, 4, 4, 1, "f32")
+    n = torch.full((128,), 520, dtype=torch.int32)
+    n[5], n[77] = 300, 0
+    many = _scan_all(v, dy, dlast, n)
+    shared = ("A", "D", "dt_bias")
+    total = {k: torch.zeros_like(many["d" + k], dtype=torch.float64) for k in shared}
+    for b in range(128):
+        one = _scan_all({k: t if k in shared else t[b:b + 1] for k, t in v.items()}, dy[b:b + 1], dlast[b:b + 1], n[b:b + 1])
+        for k in one:
+            if k[1:] in shared:
+                total[k[1:]] += one[k].double()
+            else:
+                # both are within 52 + N + 3 L roundings of the exact states and adjoints, each met at most twice
+                assert (many[k][b:b + 1] - one[k]).norm() <= 4 * (56 + 3 * 520) * 2.0 ** -24 * (one[k].norm() + 1e-3), (b, k)
+    for k in shared:
+        assert (many["d" + k].double() - total[k]).norm() <= 4 * (56 + 3 * 520) * 2.0 ** -24 * total[k].norm(), k
+
+
 def test_steep_and_flat_decay():
     """exp(delta A) from 1 (delta = 0: softplus of -200) to 0 (delta A below the range of fp32)."""
     v, dy, dlast = _inputs(1, 2, 40, 16, 8, 1, "f32")

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     // separate objects, not one array: the compiler then knows that reads of one do not wait for loads into the others
     __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * 64], lds1[(BM + BN) * 64], lds2[(BM + BN) * 64], lds3[(BM + BN) * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-    // consecutive workgroups go to the 8 dies in turn: give each die a contiguous part of the tiles, walked 8 rows of tiles deep
+    // consecutive workgroups go to the 8 dies in turn: give each die a contiguous part of the tiles, walked 4 rows of tiles deep
     int id = blockIdx.x;
     const int tiles = g.mt * g.nt, total = tiles * g.splits;
     {
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     }
     const int split = id / tiles;
     id %= tiles;
-    const int deep = 8, band = id / (deep * g.nt), high = min(deep, g.mt - band * deep);
+    const int deep = 4, band = id / (deep * g.nt), high = min(deep, g.mt - band * deep);
     const int m0 = (band * deep + (id % (deep * g.nt)) % high) * BM, nt = (id % (deep * g.nt)) / high;
     const int n0 = nt * (GATED ? BN / 2 : BN);
     const int kt0 = (int)((long long)g.ktiles * split / g.splits), kt1 = (int)((long long)g.ktiles * (split + 1) / g.splits);

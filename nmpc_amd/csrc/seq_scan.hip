@@ -26,6 +26,7 @@ struct ScanDev {
     nmpc_scan_args a;
     int nblk, per;                     // channel blocks of a group, channels of a group
     int ntile, nch, tpc;               // tiles; chunks (parts of the time axis that run side by side) and tiles of a chunk
+    int slots;                         // forward: the time axis in slots of a workgroup
     float *xin, *dsum;                 // [nb][nch][D][4P] state before a chunk; [nb][nch][D] sum of delta over it
     float *pA, *pDb, *pBC;             // partial sums (backward)
 };
@@ -340,6 +341,171 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : P == 2 ? 2 : 3) void sca
     } else if (a.last && at.chunk == s.nch - 1) {
         store_states(a.last + ((long long)at.b * a.D + ch) * a.N, a.N, q, x);
     }
+}
+
+// The scan with the time axis cut inside a workgroup: each of its four waves owns 16 of 64 steps of the same 64 / P channels.  A wave
+// first scans its steps from zero, keeping their decays in registers, the waves trade end states and total decays through LDS, and
+// each scans again from the state it now knows - without the exponentials: 8.5 instead of 6.5 slots a state and step, but no pass over
+// the samples before.  All staging is the wave's own; one barrier per 64 steps.
+template <typename T, int P, int V>
+__global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_slots_kernel(ScanDev s) {
+    constexpr int CH = 64 / P, S = Steps<P>::S, R = SCAN_SAVE, SLOTS = 4;
+    constexpr int COLS = CH / V, STEP = 64 / COLS, PER = R / STEP, NB = R * 4 * P / 64;
+    static_assert(R % STEP == 0 && 64 % COLS == 0, "whole rows");
+    __shared__ __attribute__((aligned(16))) float2 sDX[SLOTS][R][CH];
+    __shared__ __attribute__((aligned(16))) float sB[SLOTS][R][4 * P], sC[SLOTS][R][4 * P], sY[SLOTS][R][CH];
+    __shared__ __attribute__((aligned(16))) float ends[2][SLOTS][64][8];     // end state and total decay of every lane, in turn
+    const nmpc_scan_args& a = s.a;
+    // workgroups go to the 8 dies in turn: neighbouring channels, which share cache lines, go to the same one
+    const int nblk = (s.per + CH - 1) / CH, nx = a.G * nblk, total = a.nb * nx;
+    int id = blockIdx.x;
+    {
+        const int xcd = id & 7, k = id >> 3, q8 = total >> 3, r8 = total & 7;
+        id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + k;
+    }
+    const int b = id / nx, g = id % nx / nblk, first = id % nx % nblk * CH, c0 = g * s.per + first, nvalid = min(CH, s.per - first);
+    const int len = seq_length(a.lengths, b, a.L);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane / P, q = lane % P, ch = c0 + c;
+    const int cc = lane % COLS * V, row0 = lane / COLS;
+    const bool ok = c < nvalid, mine = cc < nvalid;
+    float A[4], carry[4] = {0.f, 0.f, 0.f, 0.f};
+    load_A<P>(s, ch, ok, q, A);
+    if (ok && a.start) load_states(a.start + ((long long)b * a.D + ch) * a.N, a.N, q, carry);
+    const T* u = (const T*)a.u + b * a.u_bs + c0 + cc;
+    const T* dt = (const T*)a.dt + b * a.dt_bs + c0 + cc;
+    const T* z = a.z ? (const T*)a.z + b * a.z_bs + c0 + cc : nullptr;
+    const T* B = (const T*)a.B + b * a.B_bs + (long long)g * a.N;
+    const T* C = (const T*)a.C + b * a.C_bs + (long long)g * a.N;
+    float bias[V], skip[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = a.dt_bias && mine ? a.dt_bias[c0 + cc + j] : 0.f;
+        skip[j] = a.D_skip && mine ? a.D_skip[c0 + cc + j] : 0.f;
+    }
+    Vec<T, V> nd[PER], nu[PER], nz[PER], cu[PER], cz[PER];
+    T nB[NB], nC[NB];
+    auto next = [&](int t0) {                         // this wave's 16 steps from t0 on
+        whole_or_not(nvalid == CH && t0 + R <= len, [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int t = t0 + row0 + i * STEP;
+                if (whole.value || (mine && t < len)) {
+                    nd[i] = load_vec<T, V>(dt + (long long)t * a.dt_ts);
+                    nu[i] = load_vec<T, V>(u + (long long)t * a.u_ts);
+                    if (z) nz[i] = load_vec<T, V>(z + (long long)t * a.z_ts);
+                }
+            }
+        });
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int e = lane + i * 64, t = t0 + e / (4 * P), n = e % (4 * P);
+            const bool in = t < len && n < a.N;
+            nB[i] = in ? B[(long long)t * a.B_ts + n] : (T)0.f;
+            nC[i] = in ? C[(long long)t * a.C_ts + n] : (T)0.f;
+        }
+    };
+    next(w * R);
+    for (int tile = 0; tile * SLOTS * R < a.L; ++tile) {
+        const int t0 = (tile * SLOTS + w) * R;
+        whole_or_not(nvalid == CH && t0 + R <= len, [&](auto whole) {
+            float d[PER][V];
+            deltas(d, nd, bias, a.softplus);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                float du[V];
+                const bool in = whole.value || (mine && t0 + row0 + i * STEP < len);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    du[j] = in ? d[i][j] * (float)nu[i].v[j] : 0.f;
+                    d[i][j] = in ? d[i][j] : 0.f;
+                }
+                put_pairs<V>(&sDX[w][row0 + i * STEP][cc], d[i], du);
+                cu[i] = nu[i];
+                cz[i] = nz[i];
+            }
+        });
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            (&sB[w][0][0])[lane + i * 64] = (float)nB[i];
+            (&sC[w][0][0])[lane + i * 64] = (float)nC[i];
+        }
+        __builtin_amdgcn_wave_barrier();              // the wave's own LDS operations are served in order
+        next(t0 + SLOTS * R);
+        float es[R][4], x[4] = {0.f, 0.f, 0.f, 0.f}, total_d = 0.f;
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+            const float2 dx = sDX[w][t][c];
+            float b4[4];
+            load_four(&sB[w][t][4 * q], b4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                es[t][i] = __builtin_amdgcn_exp2f(dx.x * A[i]);
+                x[i] = es[t][i] * x[i] + dx.y * b4[i];
+            }
+            total_d += dx.x;
+        }
+        float (*end)[64][8] = ends[tile & 1];
+        store_four(end[w][lane], x);
+        {
+            float decay[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) decay[i] = __builtin_amdgcn_exp2f(total_d * A[i]);
+            store_four(end[w][lane] + 4, decay);
+        }
+        __syncthreads();                              // (the other half of `ends` is free again: everyone is past its reads)
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+            float xe[4], de[4];
+            load_four(end[k][lane], xe);
+            load_four(end[k][lane] + 4, de);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = k == w ? carry[i] : x[i];
+                carry[i] = de[i] * carry[i] + xe[i];
+            }
+        }
+        if (a.saved && ok && t0 < a.L)
+            store_four((float*)a.saved + (((long long)b * ((a.L + R - 1) / R) + t0 / R) * a.D + ch) * (4 * P) + 4 * q, x);
+#pragma unroll
+        for (int t4 = 0; t4 < R; t4 += S) {
+            float y[S];
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+                const int t = t4 + k;
+                const float dx = sDX[w][t][c].y;
+                float b4[4], c4[4];
+                load_four(&sB[w][t][4 * q], b4);
+                load_four(&sC[w][t][4 * q], c4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = es[t][i] * x[i] + dx * b4[i];
+                y[k] = c4[0] * x[0] + c4[1] * x[1] + c4[2] * x[2] + c4[3] * x[3];
+            }
+            const float r = sum_steps<P>(y, lane);
+            if (P <= 4 || q < 4) sY[w][t4 + (q & 3)][c] = r;
+        }
+        __builtin_amdgcn_wave_barrier();
+        T* yo = (T*)a.y + ((long long)b * a.L + t0) * a.D + c0 + cc;
+        whole_or_not(nvalid == CH && t0 + R <= len, [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int t = row0 + i * STEP;
+                if (!whole.value && (!mine || t0 + t >= a.L)) continue;
+                const bool in = whole.value || t0 + t < len;
+                Vec<T, V> o;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v = sY[w][t][cc + j] + skip[j] * (float)cu[i].v[j];
+                    if (z) {
+                        const float zz = (float)cz[i].v[j];
+                        v *= zz * sigmoid(zz);
+                    }
+                    o.v[j] = (T)(in ? v : 0.f);
+                }
+                store_vec(yo + (long long)t * a.D, o);
+            }
+        });
+    }
+    if (ok && a.last && w == 0) store_states(a.last + ((long long)b * a.D + ch) * a.N, a.N, q, carry);
 }
 
 // From the chunks' summaries to the state before every chunk (REVERSE: the adjoint behind every chunk), in place.
@@ -775,7 +941,16 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanDev s) {
 
 static int scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
-static void scan_plan(ScanDev& s) {
+// How a pass runs: whole sequences one tile after the other, the time axis in slots of a workgroup (forward only), or in chunks with a
+// summary pass before; the least of three estimated times.  Each is the longer of the steps that follow one another and of the work at the
+// rate of a full chip (us a state and step; bf16, 16 states).  Measured, in us:                       whole   slots   chunks
+//   forward   1 x 8192 x 2048 channels (268 M states and steps)                                         1025     400      162
+//             2 x 2048 x 2048                                                                                    104       85
+//             4 x 2048 x 2048                                                                            262     122      143
+//             8 x 2048 x 2048                                                                                    221      275
+//             8 x 2048 x 4096                                                                            372     413      541
+//   backward  4 x 2048 x 2048                                                                            880              350
+static void scan_plan(ScanDev& s, bool backward) {
     const nmpc_scan_args& a = s.a;
     const int P = scan_lanes(a.N), CH = SCAN_THREADS / P;
     s.per = a.D / a.G;
@@ -783,19 +958,20 @@ static void scan_plan(ScanDev& s) {
     s.ntile = a.L > 0 ? (a.L + SCAN_T - 1) / SCAN_T : 0;
     s.nch = 1;
     s.tpc = s.ntile;
-    // Workgroups of whole sequences alone fill the chip from about 512 on (two a CU).  With fewer the time axis is cut into chunks, at the
-    // price of a pass that summarises each chunk: 3.6 of 5.6 ps a channel and step at N = 16.  bf16, 16 states: 1 x 8192 x 2048 takes 1025 us
-    // whole, 172 us with 512 workgroups, 160 us with 1024 and 157 us with 2048; 4 x 2048 x 2048 262, 164, 150 and 140 us (1 x 2048 x 2048: 248,
-    // 55, 56 and 67 us); 8 x 2048 x 4096 (512 workgroups whole) 372 us whole, 540 us in chunks.  A tile takes 4 us one after the other, the
-    // summary 2.6 us a tile and 8 us in launches: short sequences stay whole.
-    const long long base = (long long)a.nb * a.G * s.nblk, target = 1024;
-    if (base > 0 && base * 2 <= target && s.ntile > 1) {
-        const long long want = (target + base - 1) / base;
-        const int n = want < s.ntile ? (int)want : s.ntile, tpc = (s.ntile + n - 1) / n;
-        if (tpc * 6.6 + 8 < s.ntile * 4.0) {
-            s.tpc = tpc;
-            s.nch = (s.ntile + tpc - 1) / tpc;
-        }
+    s.slots = 0;
+    const long long base = (long long)a.nb * a.G * s.nblk;
+    if (base == 0 || s.ntile == 0) return;
+    const double work = (double)a.nb * a.D * a.L * 4 * P * 1e-6;
+    const long long want = (1024 + base - 1) / base;            // chunks that fill the chip: four workgroups a CU
+    const int n = want < s.ntile ? (int)want : s.ntile, tpc = (s.ntile + n - 1) / n;
+    const double whole = std::max((backward ? 13.7 : 4.0) * s.ntile, (backward ? 1.03 : 0.35) * work);
+    const double slots = backward ? 1e30 : std::max(3.0 * ((a.L + 63) / 64), 0.45 * work);
+    const double chunks = n > 1 ? std::max((backward ? 17.0 : 6.6) * tpc, (backward ? 1.29 : 0.58) * work) + 10.0 : 1e30;
+    if (slots < whole && slots <= chunks) {
+        s.slots = 1;
+    } else if (chunks < whole) {
+        s.tpc = tpc;
+        s.nch = (s.ntile + tpc - 1) / tpc;
     }
 }
 
@@ -823,6 +999,13 @@ static unsigned long long scan_workspace(ScanDev& s, bool backward, char* base) 
     return off;
 }
 
+// the number of workgroups of a pass, 0 if a launch cannot have them
+static unsigned scan_grid(const ScanDev& s) {
+    const int CH = (s.slots ? 64 : SCAN_THREADS) / scan_lanes(s.a.N);
+    const long long blocks = (long long)s.a.nb * (s.slots ? 1 : s.nch) * s.a.G * ((s.per + CH - 1) / CH);
+    return blocks < (1 << 24) ? (unsigned)blocks : 0;
+}
+
 static int scan_check(const char* what, const nmpc_scan_args* a) {
     NMPC_REQUIRE(a, "%s: null argument", what);
     NMPC_REQUIRE(a->struct_size == (int)sizeof(nmpc_scan_args), "%s: struct of %d bytes, the library's has %d", what, a->struct_size,
@@ -832,8 +1015,7 @@ static int scan_check(const char* what, const nmpc_scan_args* a) {
     NMPC_REQUIRE(a->N >= 1 && a->N <= 64, "%s: %d states a channel (1..64)", what, a->N);
     NMPC_REQUIRE(a->G >= 1 && a->D % a->G == 0, "%s: %d groups do not divide %d channels", what, a->G, a->D);
     // a launch has fewer than 2^32 threads
-    NMPC_REQUIRE((long long)a->nb * a->D * 64 < (1ll << 31) && (long long)a->nb * (a->D / 16 + a->G) * (a->L / SCAN_T + 1) < (1ll << 23),
-                 "%s: too many elements for one launch", what);
+    NMPC_REQUIRE((long long)a->nb * a->D * 64 < (1ll << 32), "%s: too many channels for one launch", what);
     // a thread's offset within 16 rows is kept in 32 bits
     const long long most = 1ll << 24;
     NMPC_REQUIRE(a->D <= most && a->u_ts >= 0 && a->u_ts <= most && a->dt_ts >= 0 && a->dt_ts <= most && (!a->z || (a->z_ts >= 0 && a->z_ts <= most)) &&
@@ -863,7 +1045,7 @@ extern "C" unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D
     if (nb <= 0 || L < 0 || D <= 0 || N <= 0 || N > 64 || G <= 0 || D % G) return 0;
     ScanDev s = {};
     s.a.nb = nb; s.a.L = L; s.a.D = D; s.a.N = N; s.a.G = G;
-    scan_plan(s);
+    scan_plan(s, backward != 0);
     return scan_workspace(s, backward != 0, nullptr);
 }
 
@@ -874,15 +1056,22 @@ extern "C" int nmpc_lpv_scan(const nmpc_scan_args* args, void* stream) {
     const nmpc_scan_args& a = s.a;
     if (a.nb == 0) return 0;
     NMPC_REQUIRE(a.A && (a.L == 0 || (a.u && a.dt && a.B && a.C && a.y)), "nmpc_lpv_scan: null argument");
-    scan_plan(s);
+    scan_plan(s, false);
     const unsigned long long need = scan_workspace(s, false, (char*)a.workspace);
     NMPC_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), "nmpc_lpv_scan: workspace of %llu bytes, %llu needed", a.workspace_bytes, need);
-    const unsigned grid = (unsigned)(a.nb * (long long)s.nch * a.G * s.nblk);
+    const unsigned grid = scan_grid(s);
+    NMPC_REQUIRE(grid || a.nb == 0, "nmpc_lpv_scan: too many sequences and channels for one launch");
     const hipStream_t st = (hipStream_t)stream;
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
             constexpr int V_ = P_ == 16 ? 1 : 2;          // 16 channels: fewer pairs than a tile has rows for
             const bool pairs = scan_pairs<T_>(s) && vec_ok<T_>(a.y, 0, 0, 2);
+            if (s.slots) {
+                if (pairs) scan_slots_kernel<T_, P_, V_><<<grid, SCAN_THREADS, 0, st>>>(s);
+                else scan_slots_kernel<T_, P_, 1><<<grid, SCAN_THREADS, 0, st>>>(s);
+                NMPC_HIP_CHECK(hipGetLastError());
+                return 0;
+            }
             if (s.nch > 1) {
                 if (pairs) scan_fwd_kernel<T_, P_, V_, true><<<grid, SCAN_THREADS, 0, st>>>(s);
                 else scan_fwd_kernel<T_, P_, 1, true><<<grid, SCAN_THREADS, 0, st>>>(s);
@@ -906,10 +1095,11 @@ extern "C" int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream) {
                  "nmpc_lpv_scan_bwd: null argument");
     NMPC_REQUIRE(!a.D_skip || a.dD, "nmpc_lpv_scan_bwd: D needs dD");
     NMPC_REQUIRE(!a.dt_bias || a.ddt_bias, "nmpc_lpv_scan_bwd: dt_bias needs ddt_bias");
-    scan_plan(s);
+    scan_plan(s, true);
     const unsigned long long need = a.nb > 0 ? scan_workspace(s, true, (char*)a.workspace) : 0;
     NMPC_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), "nmpc_lpv_scan_bwd: workspace of %llu bytes, %llu needed", a.workspace_bytes, need);
-    const unsigned grid = (unsigned)(a.nb * (long long)s.nch * a.G * s.nblk);
+    const unsigned grid = scan_grid(s);
+    NMPC_REQUIRE(grid || a.nb == 0, "nmpc_lpv_scan: too many sequences and channels for one launch");
     const hipStream_t st = (hipStream_t)stream;
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
@@ -941,7 +1131,7 @@ extern "C" int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream) {
     const nmpc_scan_args& a = s.a;
     if (a.nb == 0) return 0;
     NMPC_REQUIRE(a.A && a.u && a.dt && a.B && a.C && a.y && a.last, "nmpc_lpv_scan_step: null argument");
-    scan_plan(s);
+    scan_plan(s, false);
     NMPC_DTYPE_SWITCH(a.dtype, {
         NMPC_P_SWITCH(a.N, {
             const unsigned grid = (unsigned)(((long long)a.nb * a.D * P_ + 255) / 256);

@@ -132,10 +132,12 @@ def test_long_records(nb, steps, d, n, dtype, lengths):
     _check(v, dy, dlast, True, lengths)
 
 
-def test_chunks_of_several_tiles():
-    """128 sequences of 17 tiles are cut into chunks of three tiles (the last of two), a sequence alone into chunks of one."""
-    v, dy, dlast = _inputs(2, 128, 520, 4, 4, 1, "f32")
-    n = torch.full((128,), 520, dtype=torch.int32)
+@pytest.mark.parametrize("steps", [520, 1030])
+def test_chunks_of_several_tiles(steps):
+    """128 sequences of 17 or 33 tiles are cut into chunks of three or five tiles (the last of fewer) or slots, a sequence alone
+    into chunks of one tile."""
+    v, dy, dlast = _inputs(2, 128, steps, 4, 4, 1, "f32")
+    n = torch.full((128,), steps, dtype=torch.int32)
     n[5], n[77] = 300, 0
     many = _scan_all(v, dy, dlast, n)
     shared = ("A", "D", "dt_bias")
@@ -147,9 +149,15 @@ def test_chunks_of_several_tiles():
                 total[k[1:]] += one[k].double()
             else:
                 # both are within 52 + N + 3 L roundings of the exact states and adjoints, each met at most twice
-                assert (many[k][b:b + 1] - one[k]).norm() <= 4 * (56 + 3 * 520) * 2.0 ** -24 * (one[k].norm() + 1e-3), (b, k)
+                assert (many[k][b:b + 1] - one[k]).norm() <= 4 * (56 + 3 * steps) * 2.0 ** -24 * (one[k].norm() + 1e-3), (b, k)
     for k in shared:
-        assert (many["d" + k].double() - total[k]).norm() <= 4 * (56 + 3 * 520) * 2.0 ** -24 * total[k].norm(), k
+        assert (many["d" + k].double() - total[k]).norm() <= 4 * (56 + 3 * steps) * 2.0 ** -24 * total[k].norm(), k
+
+
+def test_many_sequences_and_channels():
+    """Enough of both that whole sequences fill the chip."""
+    v, dy, dlast = _inputs(4, 120, 40, 1000, 4, 2, "f16")
+    _check(v, dy, dlast, True, [40 - i % 41 for i in range(120)], grads=False)
 
 
 def test_steep_and_flat_decay():

@@ -306,7 +306,7 @@ int nmpc_causal_conv_step(int dtype, int nb, int D, int W, void* window, const v
  * nmpc_lpv_scan_step: one sample of every sequence, u / dt / z [nb][D], B / C [nb][G][N] (_ts unused); `last` is the state,
  * read and replaced.
  * workspace: nmpc_lpv_scan_workspace_bytes (0 for some sizes), contents need not be preserved; calls that overlap in time
- * need one each. */
+ * need one each.  saved and workspace start on 16 bytes.  Strides between steps are 0..2^24 elements. */
 typedef struct nmpc_scan_args {
     int struct_size;                     /* sizeof(nmpc_scan_args) of the caller's header; checked */
     int dtype, nb, L, D, N, G, softplus;
@@ -335,8 +335,9 @@ int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream);
  * h[M,F], all of one element type; row strides x_ld, wg_ld = wu_ld, dh_ld in elements, rows contiguous, outputs contiguous.
  * pre (NULL = no gradient wanted): fp32 [2][M][F], both projections before the activation, for _bwd.
  * _bwd: dh -> dx[M,K], dwg / dwu[F,K].  workspace: nmpc_gated_ffn_workspace_bytes (0 for some sizes; copy = 1 unless x and the
- * weights start on 16 bytes and have row strides of whole 16 bytes), contents need not be preserved; calls that overlap in
- * time need one each. */
+ * weights start on 16 bytes and have row strides of whole 16 bytes), contents need not be preserved; it starts on 16 bytes;
+ * calls that overlap in time need one each.  dG and dU (dh times the other factor and the slope) are rounded to the element
+ * type once, as operands of the gradients' products: in fp16 they have that type's range. */
 unsigned long long nmpc_gated_ffn_workspace_bytes(int dtype, int M, int K, int F, int backward, int copy);
 int nmpc_gated_ffn(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld, const void* wu,
                    long long wu_ld, int act, void* h, float* pre, void* workspace, unsigned long long workspace_bytes, void* stream);

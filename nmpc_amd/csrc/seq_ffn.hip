@@ -45,6 +45,7 @@ struct NtArgs {
     float* part;                       // fp32 partial products [splits][M][N] instead of out
     int splits;
     int mt, nt;                        // tiles
+    int wide;                          // results may be stored in pieces of 16 bytes: rows of whole groups of eight, aligned
 };
 
 template <typename T>
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     constexpr int PER = (BM + BN) * 64 / 8192;
     static_assert(2 * PER >= WAVES, "room for the results");
     float* stage = reinterpret_cast<float*>(wave < PER ? lds0 : lds1) + (wave % PER) * 2048;
-    const bool wide = g.N % 8 == 0;
+    const bool wide = g.wide;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -610,6 +611,7 @@ static int run_product(NtArgs g, hipStream_t st) {
     const Shape shape = product_shape<T>(g.M, cols, g.ktiles, !GATED && g.part);
     g.splits = shape.splits;
     if (g.splits == 1) g.part = nullptr;
+    g.wide = g.N % 8 == 0 && ((uintptr_t)g.out | (uintptr_t)g.out1 | (uintptr_t)g.pre) % 16 == 0;
     const int bm = shape.large ? 256 : 128, bn = shape.large ? 256 : 128;
     g.mt = (g.M + bm - 1) / bm;
     g.nt = (g.N + (GATED ? bn / 2 : bn) - 1) / (GATED ? bn / 2 : bn);
@@ -749,6 +751,7 @@ extern "C" int nmpc_gated_ffn(int dtype, int M, int K, int F, const void* x, lon
     if (M == 0) return 0;
     NMPC_REQUIRE(x && wg && wu && h, "nmpc_gated_ffn: null argument");
     NMPC_REQUIRE(wg_ld == wu_ld, "nmpc_gated_ffn: the weight matrices have different row strides");
+    NMPC_REQUIRE((uintptr_t)workspace % 16 == 0, "nmpc_gated_ffn: the workspace starts on 16 bytes");
     NMPC_DTYPE_SWITCH(dtype, { return run_forward<T_>(M, K, F, x, x_ld, wg, wu, wg_ld, act, h, pre, (char*)workspace, workspace_bytes, (hipStream_t)stream); })
     return 0;
 }
@@ -759,6 +762,7 @@ extern "C" int nmpc_gated_ffn_bwd(int dtype, int M, int K, int F, const void* x,
     if (ffn_check("nmpc_gated_ffn_bwd", dtype, M, K, F, act)) return 1;
     NMPC_REQUIRE(dwg && dwu && (M == 0 || (x && wg && wu && pre && dh && dx)), "nmpc_gated_ffn_bwd: null argument");
     NMPC_REQUIRE(wg_ld == wu_ld, "nmpc_gated_ffn_bwd: the weight matrices have different row strides");
+    NMPC_REQUIRE((uintptr_t)workspace % 16 == 0, "nmpc_gated_ffn_bwd: the workspace starts on 16 bytes");
     NMPC_DTYPE_SWITCH(dtype, { return run_backward<T_>(M, K, F, x, x_ld, wg, wu, wg_ld, act, pre, dh, dh_ld, dx, dwg, dwu, (char*)workspace, workspace_bytes, (hipStream_t)stream); })
     return 0;
 }

@@ -1018,8 +1018,10 @@ static int scan_check(const char* what, const nmpc_scan_args* a) {
     NMPC_REQUIRE((long long)a->nb * a->D * 64 < (1ll << 32), "%s: too many channels for one launch", what);
     // a thread's offset within 16 rows is kept in 32 bits
     const long long most = 1ll << 24;
-    NMPC_REQUIRE(a->D <= most && a->u_ts >= 0 && a->u_ts <= most && a->dt_ts >= 0 && a->dt_ts <= most && (!a->z || (a->z_ts >= 0 && a->z_ts <= most)) &&
-                 (!a->dy || (a->dy_ts >= 0 && a->dy_ts <= most)), "%s: strides between steps of 0..2^24 elements", what);
+    auto fits = [&](const void* p, long long ts) { return !p || a->L <= 1 || (ts >= 0 && ts <= most); };
+    NMPC_REQUIRE(a->D <= most && fits(a->u, a->u_ts) && fits(a->dt, a->dt_ts) && fits(a->z, a->z_ts) && fits(a->dy, a->dy_ts),
+                 "%s: strides between steps of 0..2^24 elements", what);
+    NMPC_REQUIRE(((uintptr_t)a->saved | (uintptr_t)a->workspace) % 16 == 0, "%s: saved and workspace start on 16 bytes", what);
     return 0;
 }
 

@@ -74,6 +74,12 @@ def test_forward_and_gradients(nb, steps, d, taps, dtype, act, bias, start, leng
         assert (grads[k] is None) == (k not in named), k
 
 
+def test_no_sequences():
+    y, window, saved = nmpc_amd.causal_conv_fwd(torch.zeros(0, 5, 8, device="cuda"), torch.ones(8, 3, device="cuda"), torch.ones(8, device="cuda"))
+    grads = nmpc_amd.causal_conv_bwd(saved, torch.zeros(0, 5, 8, device="cuda"))
+    assert y.shape == (0, 5, 8) and window.shape == (0, 2, 8) and not grads["dw"].any() and not grads["dbias"].any()
+
+
 def test_padding_is_never_read():
     u, w, b, s, _, dy, dwin = _inputs(3, 3, 40, 64, 4, torch.float32, True, True, None)
     n = torch.tensor([0, 5, 33], dtype=torch.int32)

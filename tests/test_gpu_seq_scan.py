@@ -214,6 +214,27 @@ def test_no_steps():
     assert not out["dA"].any() and not out["dD"].any() and not out["ddt_bias"].any()
 
 
+def test_no_sequences():
+    v, dy, dlast = _inputs(8, 0, 7, 12, 16, 2, "bf16")
+    out = _scan_all(v, dy, dlast)
+    assert out["y"].shape == (0, 7, 12) and out["last"].shape == (0, 12, 16) and out["dB"].shape == (0, 7, 2, 16)
+    assert not out["dA"].any() and not out["dD"].any() and not out["ddt_bias"].any()
+
+
+def test_single_step_of_a_far_stride():
+    """The stride between steps of a single step means nothing, however large; one that would be used and does not fit is refused."""
+    v, dy, dlast = _inputs(8, 2, 1, 8, 4, 1, "f32")
+    want = _scan_all(v, dy, dlast)
+    far = {k: gpu(t) if t is None or k not in ("u", "dt", "z") else t.cuda().as_strided(t.shape, (8, 1 << 30, 1)) for k, t in v.items()}
+    got = _scan_all(far, dy, dlast)
+    assert all(torch.equal(want[k], got[k]) for k in want)
+    u = torch.zeros(1, device="cuda").as_strided((1, 2, 8), (0, 0, 0))
+    far = torch.empty((1 << 24) + 16, device="cuda").as_strided((1, 2, 8), (0, (1 << 24) + 1, 1))
+    B = torch.zeros(1, 2, 1, 4, device="cuda")
+    with pytest.raises(nmpc_amd.NmpcError, match="strides"):
+        nmpc_amd.lpv_scan(far, u, torch.zeros(8, 4, device="cuda"), B, B)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strided_parts_of_wider_tensors(dtype):
     g = rng(3)

@@ -135,6 +135,9 @@ def test_scan_abi(tmp_path):
                dict(workspace=p, workspace_bytes=16)):
         at, hold = args(**kw)
         assert L.nmpc_lpv_scan_bwd(at, None) != 0 and L.nmpc_last_error(), kw
+    for kw in (dict(saved=p + 4), dict(workspace=p + 8, workspace_bytes=1 << 30), dict(u_ts=-1), dict(z=p, dz=p, z_ts=1 << 25)):
+        at, hold = args(**kw)
+        assert L.nmpc_lpv_scan_bwd(at, None) != 0 and b"nmpc_lpv_scan_bwd" in L.nmpc_last_error(), kw
     for kw in (dict(last=None), dict(u=None), dict(y=None)):
         at, hold = args(**kw)
         assert L.nmpc_lpv_scan_step(at, None) != 0, kw

@@ -39,6 +39,9 @@ __device__ __forceinline__ float softplus(float x) {
     return fmaxf(x, 0.f) + 2.f * s * r;
 }
 
+// What many steps do to a state, 2^x: an unstable mode's growth over them stays finite, so that a state of zero stays zero.
+__device__ __forceinline__ float decay_of(float x) { return fminf(__builtin_amdgcn_exp2f(x), 3.4e38f); }
+
 template <int CTRL, int BANKS = 0xf>
 __device__ __forceinline__ float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, BANKS, true));
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_slots_kerne
         {
             float decay[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) decay[i] = __builtin_amdgcn_exp2f(total_d * A[i]);
+            for (int i = 0; i < 4; ++i) decay[i] = decay_of(total_d * A[i]);
             store_four(end[w][lane] + 4, decay);
         }
         __syncthreads();                              // (the other half of `ends` is free again: everyone is past its reads)
@@ -525,7 +528,7 @@ __global__ __launch_bounds__(256) void scan_chunks_kernel(ScanDev s, int NP) {
         float* p = s.xin + (at * a.D + ch) * NP + n;
         const float own = *p;
         *p = x;
-        x = __builtin_amdgcn_exp2f(A * s.dsum[at * a.D + ch]) * x + own;
+        x = decay_of(A * s.dsum[at * a.D + ch]) * x + own;
     }
 }
 
@@ -1012,6 +1015,7 @@ static int scan_check(const char* what, const nmpc_scan_args* a) {
                  (int)sizeof(nmpc_scan_args));
     NMPC_REQUIRE(a->dtype >= NMPC_F32 && a->dtype <= NMPC_F16, "%s: unknown element type %d", what, a->dtype);
     NMPC_REQUIRE(a->nb >= 0 && a->L >= 0 && a->D >= 1, "%s: bad sizes (%d sequences, %d steps, %d channels)", what, a->nb, a->L, a->D);
+    NMPC_REQUIRE(a->L <= 1 << 30, "%s: at most 2^30 steps", what);
     NMPC_REQUIRE(a->N >= 1 && a->N <= 64, "%s: %d states a channel (1..64)", what, a->N);
     NMPC_REQUIRE(a->G >= 1 && a->D % a->G == 0, "%s: %d groups do not divide %d channels", what, a->G, a->D);
     // a launch has fewer than 2^32 threads
@@ -1039,12 +1043,12 @@ static int scan_check(const char* what, const nmpc_scan_args* a) {
 using namespace nmpc;
 
 extern "C" unsigned long long nmpc_lpv_scan_saved_bytes(int nb, int L, int D, int N) {
-    if (nb <= 0 || L <= 0 || D <= 0 || N <= 0 || N > 64) return 0;
+    if (nb <= 0 || L <= 0 || L > 1 << 30 || D <= 0 || N <= 0 || N > 64) return 0;
     return (unsigned long long)nb * ((L + SCAN_SAVE - 1) / SCAN_SAVE) * D * 4 * scan_lanes(N) * sizeof(float);
 }
 
 extern "C" unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D, int N, int G, int backward) {
-    if (nb <= 0 || L < 0 || D <= 0 || N <= 0 || N > 64 || G <= 0 || D % G) return 0;
+    if (nb <= 0 || L < 0 || L > 1 << 30 || D <= 0 || N <= 0 || N > 64 || G <= 0 || D % G) return 0;
     ScanDev s = {};
     s.a.nb = nb; s.a.L = L; s.a.D = D; s.a.N = N; s.a.G = G;
     scan_plan(s, backward != 0);

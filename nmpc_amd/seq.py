@@ -17,6 +17,7 @@ from ._lib import NmpcError, lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "tanh": 3, "sigmoid": 4}
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 _Tensor = torch.Tensor
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -84,11 +85,11 @@ def _lengths(what, t, nb):
         return None
     if not isinstance(t, _Tensor) or t.shape != (nb,):
         _fail(what, "lengths must be [%d], got %s", nb, _got(t))
-    if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+    if t.dtype not in _INTEGERS:
         _fail(what, "lengths are %s, expected integers", t.dtype)
     if t.dtype is torch.int32 and t.is_contiguous():
         return t
-    if t.element_size() > 4:                                   # values past int32 would wrap around: those above any length are one
+    if t.dtype is torch.int64:                                 # values past int32 would wrap around: those above any length are one
         t = t.clamp(-1, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 

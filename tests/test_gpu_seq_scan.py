@@ -183,6 +183,36 @@ def test_steep_and_flat_decay():
     assert all(torch.isfinite(t).all() for t in n.values() if t is not None)
 
 
+@pytest.mark.parametrize("nb,steps,d", [(2, 70, 8), (2, 1100, 24), (8, 500, 2048)])
+def test_growing_modes_at_rest(nb, steps, d):
+    """Modes that grow by e^10 a step, past any number within a part of the time axis: a state or an adjoint of zero stays zero."""
+    v, dy, dlast = _inputs(3, nb, steps, d, 4, 1, "f32", gate=False, bias=False, start=False)
+    v["A"] = torch.full((d, 4), 10.0)
+    v["dt"] = torch.full_like(v["dt"], 1.0)
+    late = {k: None if t is None else t.clone() for k, t in v.items()}
+    late["u"][:, :-3] = 0
+    y, last, _ = nmpc_amd.lpv_scan_fwd(*[gpu(late[k]) for k in NAMES[:8]], False)
+    want, state = oracle.lpv_scan(*[None if late[k] is None else f64(late[k][:, -3:] if k in ("u", "dt", "B", "C") else late[k]) for k in NAMES[:8]], use_softplus=False)
+    assert not y[:, :-3].any()
+    m = _magnitudes({k: None if t is None else t[:, -3:] if k in ("u", "dt", "B", "C") else t for k, t in late.items()}, dy[:, -3:], dlast, False, None)
+    # the exponent 10 log2(e) is rounded once and meant to a rounding: 2 x 10 a step, three steps; else as above
+    assert_close(y[:, -3:], want, 52 + 4 + 9 + 60, m["y"], "y")
+    assert_close(last, state, 52 + 4 + 9 + 60, m["last"], "last")
+    # the adjoint: gradients of the first steps' outputs only, nothing behind them
+    v["u"] = torch.zeros_like(v["u"])
+    y, last, saved = nmpc_amd.lpv_scan_fwd(*[gpu(v[k]) for k in NAMES[:8]], False)
+    assert not y.any() and not last.any()
+    dy[:, 3:] = 0
+    got = nmpc_amd.lpv_scan_bwd(saved, gpu(dy))
+    assert all(torch.isfinite(t).all() for t in got.values() if t is not None)
+    assert not got["du"][:, 3:].any() and not got["dC"].any() and not got["dA"].any()
+    few = {k: None if t is None else leaf(t[:, :3] if k in ("u", "dt", "B", "C") else t) for k, t in v.items()}
+    yo, _ = oracle.lpv_scan(*[few[k] for k in NAMES[:8]], use_softplus=False)
+    du, = torch.autograd.grad([yo], [few["u"]], [f64(dy[:, :3])])
+    m = _magnitudes({k: None if t is None else t[:, :3] if k in ("u", "dt", "B", "C") else t for k, t in v.items()}, dy[:, :3], torch.zeros_like(dlast), False, None)
+    assert_close(got["du"][:, :3], du, 2 * (52 + 4 + 9 + 60) + 120, m["u"], "du")
+
+
 def _scan_all(v, dy, dlast, lengths=None):
     y, last, saved = nmpc_amd.lpv_scan_fwd(*[gpu(v[k]) for k in NAMES[:8]], True, gpu(v["start"]), gpu(lengths))
     return {"y": y, "last": last, **nmpc_amd.lpv_scan_bwd(saved, gpu(dy), gpu(dlast))}

@@ -30,7 +30,7 @@ def test_conv_refusals():
         (dict(w=torch.zeros(8, 4, dtype=torch.int32)), "floating"), (dict(bias=torch.zeros(7)), r"bias must be \[8\]"),
         (dict(act="gelu"), "activation"), (dict(start=torch.zeros(2, 4, 8)), "start must be"),
         (dict(start=torch.zeros(2, 3, 8).half()), "the samples are"), (dict(lengths=torch.zeros(3, dtype=torch.int32)), r"lengths must be \[2\]"),
-        (dict(lengths=torch.zeros(2)), "integers"),
+        (dict(lengths=torch.zeros(2)), "integers"), (dict(lengths=torch.zeros(2, dtype=torch.uint32)), "integers"),
     ]
     for change, text in bad:
         args = {**dict(u=u, w=w), **change}
@@ -47,6 +47,17 @@ def test_conv_refusals():
         nmpc_amd.causal_conv_bwd("saved", u)
 
 
+def test_lengths_keep_their_meaning():
+    """Integers of every width mean the same steps; those past 32 bits are above or below every length."""
+    from nmpc_amd.seq import _lengths
+    for t in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+        got = _lengths("f", torch.tensor([0, 100, 7], dtype=t), 3)
+        assert got.dtype is torch.int32 and got.tolist() == [0, 100, 7]
+    got = _lengths("f", torch.tensor([2 ** 40, -2 ** 40, 5]), 3).tolist()
+    assert got[0] == 2 ** 31 - 1 and got[1] < 0 and got[2] == 5
+    assert _lengths("f", torch.arange(8)[::2], 4).is_contiguous()
+
+
 def test_conv_abi_refusals():
     L = _lib.lib()
     buf = (ctypes.c_float * 64)()                     # never touched: every call below is refused first
@@ -54,7 +65,7 @@ def test_conv_abi_refusals():
     def fwd(dtype=0, nb=1, steps=4, d=4, taps=4, u=p, w=p, act=0, y=p):
         return L.nmpc_causal_conv(dtype, nb, steps, d, taps, u, 16, 4, w, None, act, None, None, y, None, None)
     for kw in (dict(dtype=3), dict(nb=-1), dict(steps=-1), dict(d=0), dict(taps=0), dict(taps=9), dict(u=None), dict(w=None),
-               dict(act=2), dict(y=None), dict(nb=1 << 30, steps=1 << 10)):
+               dict(act=2), dict(y=None), dict(nb=1 << 30, steps=1 << 10), dict(steps=2 ** 31 - 1, d=1)):
         assert fwd(**kw) != 0 and L.nmpc_last_error(), kw
     assert fwd(nb=0, u=None, y=None) == 0             # nothing to do
     need = L.nmpc_causal_conv_workspace_bytes(2, 40, 8, 4)
@@ -128,7 +139,7 @@ def test_scan_abi(tmp_path):
             setattr(s, k, v)
         return ctypes.addressof(s), s
     for kw in (dict(struct_size=8), dict(dtype=7), dict(nb=-1), dict(L=-1), dict(D=0), dict(N=0), dict(N=65), dict(G=3), dict(G=0), dict(A=None),
-               dict(u=None), dict(C=None), dict(y=None), dict(nb=1 << 20, D=1 << 12)):
+               dict(u=None), dict(C=None), dict(y=None), dict(nb=1 << 20, D=1 << 12), dict(L=2 ** 31 - 1, D=1)):
         at, hold = args(**kw)
         assert L.nmpc_lpv_scan(at, None) != 0 and L.nmpc_last_error(), kw
     for kw in (dict(saved=None), dict(dy=None), dict(dA=None), dict(dB=None), dict(z=p), dict(D_skip=p), dict(dt_bias=p), dict(workspace=None),

@@ -2,8 +2,12 @@
 //   dG = dh o up o act'(gate),  dU = dh o act(gate),
 //   dx = dG Wg + dU Wu,  dWg = dG' x,  dWu = dU' x.
 // Both projections of a tile are accumulated side by side, so that the activation and the product happen in registers and
-// neither projection is written (a training pass keeps both in fp32 for the gradient).  Products run on the matrix cores with
-// fp32 accumulation; dG and dU are rounded to the element type once, as operands of the next products.
+// neither projection is written (a training pass keeps both in fp32 for the gradient: kept in bf16 the gradients were off by 1.65
+// times as much).  Products run on the matrix cores with fp32 accumulation; dG and dU are rounded to the element type once, as
+// operands of the next products, which take both side by side: dx is one product over 2 F, [dWg; dWu] one of 2 F rows.
+// What bounds it: many rows the matrix cores, few rows reading the weights, a prompt of a few hundred rows the latency of its loads.
+// Measured: bf16 4096 x 2048 x 8192 forward 336 us and gradient 581 us, 0.9 PFLOP/s over a training step (the library's plain products of
+// these sizes reach 1.1 .. 1.3); fp32 4096 x 256 x 1024 training 160 us (81 TFLOP/s); bf16 1 x 2048 x 8192 12.9 us, 5.2 TB/s.
 #include <cmath>
 
 #include "seq_common.h"

@@ -9,8 +9,15 @@
 // Layout.  A lane owns four states of a channel and P = ceil(N / 4) rounded up to 1, 2, 4, 8, 16 lanes a channel (states past N
 // are zero throughout); a workgroup of 256 threads owns 256 / P channels of one group (the channels that share B and C) and walks
 // the steps in tiles of 32.  A tile's samples are staged once per element through LDS (softplus, its product with u), so that the
-// P lanes of a channel do not repeat them; B and C are read from LDS as one 16-byte access per lane.
-// What bounds it: VALU issue.  A state and step costs 2 (exp2) + 4 slots forward; the bytes are 8 a channel and step in bf16.
+// P lanes of a channel do not repeat them; B and C are read from LDS as one 16-byte access per lane; the next tile's loads are in
+// flight meanwhile.  Sequences that do not fill the chip are cut in time (scan_plan): chunks whose effect on a state, x_end =
+// exp(A sum delta) x_begin + own, is found in a pass before, or slots of a workgroup that keep their decays in registers.
+// What bounds it: VALU issue.  A state and step costs 6.5 slots forward (its exponential alone 2.5) and about 22 backward, of which
+// 6.5 are the states of a tile computed again from the one saved before it: saving every 16th state costs 1/4 byte a state and step
+// instead of 4.  Sums over the lanes of a channel and over the channels of a group trade
+// halves, so that four steps (eight values) share the stages of one.
+// Measured, bf16, 16 states: 4 x 2048 steps x 2048 channels forward 122 us, training 483 us (279 of them the main backward pass);
+// 1 x 8192 x 2048 forward 152 us; step of 64 x 4096 channels 9.5 us, 3.8 TB/s.
 #include <algorithm>
 #include <type_traits>
 

@@ -140,6 +140,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     constexpr int BM = WM * MI * 32, BN = WN * 64, WAVES = WM * WN, E = 16 / sizeof(T), BK = 64 / sizeof(T);
     constexpr int LOADS = (BM + BN) * 64 / 1024 / WAVES, AUNITS = BM / 16;
     static_assert((BM + BN) * 64 % (1024 * WAVES) == 0 && AUNITS % WAVES == 0 && (!GATED || (KA && KB)), "whole loads");
+    static_assert(KA || BM >= 128, "the exclusive or of pieces of rows k needs sixteen of them");
     // separate objects, not one array: the compiler then knows that reads of one do not wait for loads into the others
     __shared__ __attribute__((aligned(1024))) char lds0[(BM + BN) * 64], lds1[(BM + BN) * 64], lds2[(BM + BN) * 64], lds3[(BM + BN) * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -225,9 +226,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     // before a tile is read: its loads have arrived (two tiles' may still be in flight), everyone's have, and everyone has read the
     // tile whose buffer is filled next
     auto arrive = [] {
-        static_assert(LOADS == 4, "loads that may be in flight: two tiles");
+        static_assert(2 * LOADS < 16, "loads that may be in flight: two tiles");
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0078);            // vmcnt 8, lgkmcnt 0; as a builtin, so that the compiler counts with it
+        __builtin_amdgcn_s_waitcnt(0x0070 | 2 * LOADS); // vmcnt: two tiles' loads, lgkmcnt 0; as a builtin, so that the compiler counts with it
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
@@ -271,8 +272,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     // Results: 32 rows at a time through 8 KB of LDS of the wave's own, so that a lane has 8 neighbouring columns; 4-column pieces sit
     // at piece ^ (row & 15) against bank conflicts.
     constexpr int PER = (BM + BN) * 64 / 8192;
-    static_assert(2 * PER >= WAVES, "room for the results");
-    float* stage = reinterpret_cast<float*>(wave < PER ? lds0 : lds1) + (wave % PER) * 2048;
+    static_assert(4 * PER >= WAVES, "room for the results");
+    const int place = wave / PER;
+    float* stage = reinterpret_cast<float*>(place == 0 ? lds0 : place == 1 ? lds1 : place == 2 ? lds2 : lds3) + (wave % PER) * 2048;
     const bool wide = g.wide;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -551,27 +553,29 @@ static bool tiled(const void* p, long long ld, int K, bool by_k) {
 
 // Tile size and splits of a product: the choice of least estimated time.  A 256 x 256 tile has a CU for itself, two 128 x 128 tiles share
 // one; a k-tile of the large one takes 1.06 us in 16 bits and 4.0 us in fp32 (measured at 16384 x 2048 x 4096), of the small one a
-// quarter of it and a sixth more, less well used where a CU has one alone.  Every round of tiles pays for filling and draining; a split
-// contraction pays for writing and reading its partial products.
+// quarter of it and a sixth more, less well used where a CU has one alone.  Tiles of 64 x 128 (`small`: A's rows lie along k) divide few
+// rows more finely and cost 0.24 and 0.56 us a k-tile: 512 x 2048 x 2048 in bf16 19 instead of 24 us, 256 x 1024 x 4096 in fp32 42 instead
+// of 71; at 1024 x 1024 x 4096 they take 37 instead of 29 and 142 instead of 139.  Every round of tiles pays for filling and draining;
+// a split contraction pays for writing and reading its partial products.
 struct Shape {
-    bool large;
-    int splits;
+    int bm, bn, splits;
     double us;
 };
 template <typename T>
-static Shape product_shape(int M, int N, int ktiles, bool may_split) {
+static Shape product_shape(int M, int N, int ktiles, bool small, bool may_split) {
     const double ktime = sizeof(T) == 2 ? 1.06 : 4.0, fill = 4.0;
-    Shape best = {false, 1, 1e30};
-    for (int large = 0; large < 2; ++large) {
-        const int b = large ? 256 : 128;
-        const double tiles = (double)((M + b - 1) / b) * ((N + b - 1) / b);
+    Shape best = {128, 128, 1, 1e30};
+    for (int tile = small ? 0 : 1; tile < 3; ++tile) {
+        const int bm = tile == 0 ? 64 : tile == 1 ? 128 : 256, bn = tile == 2 ? 256 : 128;
+        const double tiles = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
         for (int splits = 1; splits <= (may_split ? 64 : 1) && (splits == 1 || splits * 4 <= ktiles); ++splits) {
             const double n = tiles * splits, depth = (ktiles + splits - 1) / splits;
             double t;
-            if (large) t = ceil(n / 256) * (depth * ktime + fill);
-            else t = n <= 256 ? depth * ktime * 0.25 * (sizeof(T) == 2 ? 1.25 : 1.0) + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
+            if (tile == 2) t = ceil(n / 256) * (depth * ktime + fill);
+            else if (tile == 1) t = n <= 256 ? depth * ktime * 0.25 * (sizeof(T) == 2 ? 1.25 : 1.0) + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
+            else t = ceil(n / 256) * depth * (sizeof(T) == 2 ? 0.24 : 0.56) + fill;
             if (splits > 1) t += 6.0 + (double)splits * M * N * 8 / 4.5e6;
-            if (t < best.us) best = {large != 0, splits, t};
+            if (t < best.us) best = {bm, bn, splits, t};
         }
     }
     return best;
@@ -606,23 +610,25 @@ template <typename T>
 static bool serves_few(int M, int K, int F, bool aligned) {
     if (M <= FEW_ROWS) return true;
     if ((M + 15) / 16 > 65535) return false;
-    return few_shape<T>(M, K, F, aligned).us < product_shape<T>(M, 2 * F, (K + ktile<T>() - 1) / ktile<T>(), false).us + (aligned ? 0.0 : 6.0);
+    return few_shape<T>(M, K, F, aligned).us < product_shape<T>(M, 2 * F, (K + ktile<T>() - 1) / ktile<T>(), true, false).us + (aligned ? 0.0 : 6.0);
 }
 
 template <typename T, bool GATED, bool KA, bool KB>
 static int run_product(NtArgs g, hipStream_t st) {
     const int cols = GATED ? 2 * g.N : g.N;
-    const Shape shape = product_shape<T>(g.M, cols, g.ktiles, !GATED && g.part);
+    const Shape shape = product_shape<T>(g.M, cols, g.ktiles, KA, !GATED && g.part);
     g.splits = shape.splits;
     if (g.splits == 1) g.part = nullptr;
     g.wide = g.N % 8 == 0 && ((uintptr_t)g.out | (uintptr_t)g.out1 | (uintptr_t)g.pre) % 16 == 0;
-    const int bm = shape.large ? 256 : 128, bn = shape.large ? 256 : 128;
-    g.mt = (g.M + bm - 1) / bm;
-    g.nt = (g.N + (GATED ? bn / 2 : bn) - 1) / (GATED ? bn / 2 : bn);
+    const int bn = GATED ? shape.bn / 2 : shape.bn;
+    g.mt = (g.M + shape.bm - 1) / shape.bm;
+    g.nt = (g.N + bn - 1) / bn;
     const long long grid = (long long)g.mt * g.nt * g.splits;
     NMPC_REQUIRE(grid < (1 << 22), "gated_ffn: too many tiles for one launch");
-    if (shape.large) gemm_kernel<T, 2, 4, 4, GATED, KA, KB><<<(unsigned)grid, 512, 0, st>>>(g);
-    else gemm_kernel<T, 2, 2, 2, GATED, KA, KB><<<(unsigned)grid, 256, 0, st>>>(g);
+    if (shape.bm == 256) gemm_kernel<T, 2, 4, 4, GATED, KA, KB><<<(unsigned)grid, 512, 0, st>>>(g);
+    else if (shape.bm == 64) {
+        if constexpr (KA) gemm_kernel<T, 2, 2, 1, GATED, KA, KB><<<(unsigned)grid, 256, 0, st>>>(g);
+    } else gemm_kernel<T, 2, 2, 2, GATED, KA, KB><<<(unsigned)grid, 256, 0, st>>>(g);
     if (g.splits > 1) {
         const long long blocks = ((long long)g.M * g.N + 255) / 256;
         gemm_join_kernel<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(g);
@@ -654,7 +660,7 @@ struct FfnSpace {
         }
         if (!backward) return s;
         s.rows = take(e * Mp * 2 * Fp);
-        const Shape a = product_shape<T>(M, K, 2 * Fp / kt, true), b = product_shape<T>(2 * Fp, K, Mp / kt, true);
+        const Shape a = product_shape<T>(M, K, 2 * Fp / kt, true, true), b = product_shape<T>(2 * Fp, K, Mp / kt, false, true);
         const unsigned long long pa = a.splits > 1 ? 4ull * a.splits * M * K : 0, pb = b.splits > 1 ? 4ull * b.splits * 2 * Fp * K : 0;
         s.part = take(pa > pb ? pa : pb);
         return s;

@@ -112,8 +112,12 @@ def test_strides_and_leading_dimensions(dtype, m):
         wdh = normal(g, 2 * m, 97 + off, dtype=DTYPES[dtype]).cuda()
         p = (wide[:, off:off + 64], both[:96, off:off + 64], both[96:, off:off + 64], wdh[:, off:off + 96])
         a, b = _run(*p, "silu"), _run(*[t.contiguous() for t in p], "silu")
+        # aligned and unaligned rows may take different kernels, which add in other orders: each result lies within `bound` of the
+        # exact value before its last rounding, so that two of them differ by at most twice that and their roundings
+        bound, half = _bounds(*[t.contiguous() for t in p], "silu"), torch.finfo(DTYPES[dtype]).eps / 2 * (1 + 2.0 ** -6)
         for key in a:
-            assert torch.allclose(a[key].float(), b[key].float(), rtol=2e-2 if dtype == "bf16" else 1e-5, atol=2e-2 if dtype == "bf16" else 1e-4), key
+            x64, y64 = a[key].double(), b[key].double()
+            assert ((x64 - y64).abs() <= 2 * (1 + half) * bound[key] + half * (x64.abs() + y64.abs())).all(), key
     t = x.t().contiguous().t()                                       # columns contiguous: copied
     assert torch.equal(nmpc_amd.gated_ffn(t, wg, wu), want["h"])
 

@@ -960,6 +960,8 @@ static int scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N 
 //             8 x 2048 x 2048                                                                                    221      275
 //             8 x 2048 x 4096                                                                            372     413      541
 //   backward  4 x 2048 x 2048                                                                            880              350
+//             fp32 64 x 50 x 64, 8 states, both passes called eagerly                                        58               64
+//             64 x 50 x 64 channels of 8 states, called eagerly                                             58               64
 static void scan_plan(ScanDev& s, bool backward) {
     const nmpc_scan_args& a = s.a;
     const int P = scan_lanes(a.N), CH = SCAN_THREADS / P;
@@ -976,7 +978,7 @@ static void scan_plan(ScanDev& s, bool backward) {
     const int n = want < s.ntile ? (int)want : s.ntile, tpc = (s.ntile + n - 1) / n;
     const double whole = std::max((backward ? 13.7 : 4.0) * s.ntile, (backward ? 1.03 : 0.35) * work);
     const double slots = backward ? 1e30 : std::max(3.0 * ((a.L + 63) / 64), 0.45 * work);
-    const double chunks = n > 1 ? std::max((backward ? 17.0 : 6.6) * tpc, (backward ? 1.29 : 0.58) * work) + 10.0 : 1e30;
+    const double chunks = n > 1 ? std::max((backward ? 17.0 : 6.6) * tpc, (backward ? 1.29 : 0.58) * work) + (backward ? 12.0 : 10.0) : 1e30;
     if (slots < whole && slots <= chunks) {
         s.slots = 1;
     } else if (chunks < whole) {

@@ -133,6 +133,18 @@ struct Stream {
     }
 };
 
+// zeros to rows t0 .. end of a workgroup's columns of CH channels, `nvalid` of them there, in a result [..][D]
+template <typename T, int CH, int V>
+__device__ __forceinline__ void zero_rows(T* p, int D, int t0, int end, int nvalid) {
+    constexpr int COLS = CH / V;
+    const int cc = threadIdx.x % COLS * V;
+    Vec<T, V> zero;
+#pragma unroll
+    for (int j = 0; j < V; ++j) zero.v[j] = (T)0.f;
+    if (cc < nvalid)
+        for (int t = t0 + (int)threadIdx.x / COLS; t < end; t += SCAN_THREADS / COLS) store_vec(p + (long long)t * D + cc, zero);
+}
+
 // f(true) for a tile whose steps and channels all count, f(false) otherwise
 template <typename F>
 __device__ __forceinline__ void whole_or_not(bool whole, F f) {
@@ -258,7 +270,8 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : P == 2 ? 2 : 3) void sca
         bias[j] = a.dt_bias && mine ? a.dt_bias[at.c0 + part.cc + j] : 0.f;
         skip[j] = !SUMMARY && a.D_skip && mine ? a.D_skip[at.c0 + part.cc + j] : 0.f;
     }
-    const int tile0 = at.chunk * s.tpc, tile1 = min(tile0 + s.tpc, s.ntile);
+    // tiles behind the sequence are not worked on: nothing but zeros to write
+    const int tile0 = at.chunk * s.tpc, tile2 = min(tile0 + s.tpc, s.ntile), tile1 = min(tile2, (at.len + SCAN_T - 1) / SCAN_T);
     auto whole = [&](int t0) { return at.nvalid == CH && t0 + SCAN_T <= at.len; };
     Vec<T, V> nd[PER], nu[PER], nz[PER], cu[PER], cz[PER];           // the next tile's samples, this one's
     Shared<T, P, SCAN_T> nB, nC;
@@ -344,6 +357,8 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : P == 2 ? 2 : 3) void sca
             });
         }
     }
+    if constexpr (!SUMMARY)
+        zero_rows<T, CH, V>((T*)a.y + (long long)at.b * a.L * a.D + at.c0, a.D, max(tile0, tile1) * SCAN_T, min(tile2 * SCAN_T, a.L), at.nvalid);
     if (!ok) return;
     if constexpr (SUMMARY) {
         store_four(chunk_state, x);
@@ -415,7 +430,8 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_slots_kerne
         }
     };
     next(w * R);
-    for (int tile = 0; tile * SLOTS * R < a.L; ++tile) {
+    const int tiles = (len + SLOTS * R - 1) / (SLOTS * R);    // behind the sequence there is nothing but zeros to write
+    for (int tile = 0; tile < tiles; ++tile) {
         const int t0 = (tile * SLOTS + w) * R;
         whole_or_not(nvalid == CH && t0 + R <= len, [&](auto whole) {
             float d[PER][V];
@@ -515,6 +531,7 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_slots_kerne
             }
         });
     }
+    zero_rows<T, CH, V>((T*)a.y + (long long)b * a.L * a.D + c0, a.D, tiles * SLOTS * R, a.L, nvalid);
     if (ok && a.last && w == 0) store_states(a.last + ((long long)b * a.D + ch) * a.N, a.N, q, carry);
 }
 
@@ -559,7 +576,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_summary_kernel(ScanDev 
     const Stream<T, V, PT> dt(a.dt, a.dt_bs, a.dt_ts, at.b, at.c0, part), z(a.z, a.z_bs, a.z_ts, at.b, at.c0, part),
         dy(a.dy, a.dy_bs, a.dy_ts, at.b, at.c0, part);
     const T* C = (const T*)a.C + at.b * a.C_bs + (long long)at.g * a.N;
-    const int tile0 = at.chunk * s.tpc, tile1 = min(tile0 + s.tpc, s.ntile);
+    const int tile0 = at.chunk * s.tpc, tile1 = min(min(tile0 + s.tpc, s.ntile), (at.len + SCAN_T - 1) / SCAN_T);
     auto whole = [&](int t0) { return at.nvalid == CH && t0 + SCAN_T <= at.len; };
     Vec<T, V> nd[PER], ng[PER], nz[PER];
     Shared<T, P, SCAN_T> nC;
@@ -680,7 +697,15 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_bwd_kernel(
     const T* B = (const T*)a.B + at.b * a.B_bs + (long long)at.g * a.N;
     const T* C = (const T*)a.C + at.b * a.C_bs + (long long)at.g * a.N;
     auto whole = [&](int t0) { return at.nvalid == CH && t0 + R <= at.len; };
-    const int ntile = (a.L + R - 1) / R, tile0 = at.chunk * s.tpc * (SCAN_T / R), tile1 = min(tile0 + s.tpc * (SCAN_T / R), ntile);
+    const int ntile = (a.L + R - 1) / R, tile0 = at.chunk * s.tpc * (SCAN_T / R), tile2 = min(tile0 + s.tpc * (SCAN_T / R), ntile);
+    const int tile1 = min(tile2, (at.len + R - 1) / R);       // tiles behind the sequence: zeros; their sums are not read
+    {
+        const long long seq = (long long)at.b * a.L * a.D + at.c0;
+        const int t0 = max(tile0, tile1) * R, end = min(tile2 * R, a.L);
+        zero_rows<T, CH, V>((T*)a.du + seq, a.D, t0, end, at.nvalid);
+        zero_rows<T, CH, V>((T*)a.ddt + seq, a.D, t0, end, at.nvalid);
+        if (a.z) zero_rows<T, CH, V>((T*)a.dz + seq, a.D, t0, end, at.nvalid);
+    }
     Vec<T, V> nd[PER], nu[PER], ng[PER], nz[PER], cd[PER], cg[PER], cz[PER];
     Shared<T, P, R> nB, nC;
     auto next = [&](int t0) {
@@ -882,7 +907,9 @@ __global__ __launch_bounds__(256) void scan_reduce_bc_kernel(ScanDev s, int NP) 
         const int n = (int)(id % (2 * NP));
         const long long r = id / (2 * NP);
         float v = 0.f;
-        for (int k = 0; k < s.nblk; ++k) v += s.pBC[(k * rows + r) * (2 * NP) + n];
+        const long long bt = r / a.G;
+        const bool in = !a.lengths || (int)(bt % a.L) < seq_length(a.lengths, (int)(bt / a.L), a.L);
+        for (int k = 0; in && k < s.nblk; ++k) v += s.pBC[(k * rows + r) * (2 * NP) + n];
         if (n < a.N) ((T*)a.dB)[r * a.N + n] = (T)v;
         else if (n >= NP && n - NP < a.N) ((T*)a.dC)[r * a.N + n - NP] = (T)v;
     }

@@ -124,6 +124,14 @@ def test_forward_and_gradients(nb, steps, d, n, groups, dtype, skip, gate, bias,
     _check(v, dy, dlast, softplus, lengths)
 
 
+@pytest.mark.parametrize("n", [16, 17, 23, 24, 25, 32, 47, 48, 49])
+@pytest.mark.parametrize("steps", [40, 300])
+def test_states_per_lane(n, steps):
+    """Either side of every change of lanes a channel and states a lane, whole sequences and parts of the time axis."""
+    v, dy, dlast = _inputs(n, 2, steps, 10, n, 2, "f32")
+    _check(v, dy, dlast, True, [steps, steps - 7])
+
+
 @pytest.mark.parametrize("nb,steps,d,n,dtype,lengths", [
     (1, 515, 16, 16, "f32", None), (1, 600, 10, 4, "bf16", None), (2, 430, 8, 40, "f32", [430, 129]), (3, 330, 12, 8, "f16", [0, 65, 330])])
 def test_long_records(nb, steps, d, n, dtype, lengths):

@@ -3,11 +3,11 @@
 // Gradients, with ds = dy act'(s):
 //   dline[k,c] = sum_j w[c,j] ds[k-j,c]  (+ dwindow where row k is one of the last W-1),   dw[c,j] = sum ds[t,c] line[t+j,c].
 // All of it is bound by memory: one read of u and one write of y (backward: u, dy in, du out).  A thread owns a few neighbouring
-// channels and a run of 16 steps; the W-1 rows before the run (backward: behind it) are read again by the neighbouring run, mostly
+// channels and a run of steps; the W-1 rows before the run (backward: behind it) are read again by the neighbouring run, mostly
 // from the L2 cache, and everything else of the filter stays in registers.  Arithmetic and sums are fp32.
-// Channels of a thread, measured at bf16 4 x 2048 x 4096, W = 4: forward 8 bytes 28 us (4.8 TB/s; 16 bytes 37 us: half the waves),
-// backward 4 bytes 61 us (3.3 TB/s; 8 bytes 76 us and 16 bytes 115 us: the unrolled run then takes 216 and over 256 registers).
-// Runs of 32 steps need 185 registers instead of 121 in the backward pass: 82 us.
+// Measured at bf16 4 x 2048 x 4096, W = 4.  Channels of a thread: forward 8 bytes 28 us (4.8 TB/s; 16 bytes 37 us: half the waves),
+// backward 4 bytes 48 us (4.2 TB/s; 8 bytes 61 us).  Steps of a run: forward 16 (24 .. 28 us for 16 .. 32), backward 28 (16: 58 us,
+// 24: 48, 32: 63; over ten shapes 28 is the least in seven): runs of 2^n rows of 2^m bytes meet on the same memory channels.
 #include <type_traits>
 
 #include "seq_common.h"
@@ -15,7 +15,8 @@
 namespace nmpc {
 
 constexpr int CONV_MAX_W = 8;
-constexpr int CONV_TR = 16;          // steps of one thread
+constexpr int CONV_TR = 16;          // steps of one thread, forward
+constexpr int CONV_TR_BWD = 28;      // backward
 constexpr int CONV_GROUP = 4;        // steps whose loads are in flight together
 
 struct ConvArgs {
@@ -45,6 +46,13 @@ __device__ __forceinline__ Vec<T, VEC> line_row(const T* ub, long long u_ts, con
     return z;
 }
 
+// f with the flag as a constant, so that the steps of a run are one block of code
+template <typename F>
+__device__ __forceinline__ void either(bool flag, F f) {
+    if (flag) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 template <typename T, int W, int VEC>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
     const unsigned gid = blockIdx.x * 256u + threadIdx.x;
@@ -72,15 +80,18 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
             for (int i = 0; i < VEC; ++i) win[j][i] = (float)r.v[i];
         }
     }
+    // rows of the run: a thread's own address plus multiples of the stride that are the same for all threads
+    const T* ur = ub + t0 * a.u_ts;
+    T* yr = yb + (long long)t0 * a.D;
     // all loads of a group of steps before its first store (the compiler cannot know that y is not u)
-    auto group = [&](int tg, auto whole) {
+    auto group = [&](int k0, auto whole, auto silu) {
         Vec<T, VEC> rows[CONV_GROUP];
 #pragma unroll
         for (int k = 0; k < CONV_GROUP; ++k)
-            if (whole.value || tg + k < tv) rows[k] = load_vec<T, VEC>(ub + (tg + k) * a.u_ts);
+            if (whole.value || t0 + k0 + k < tv) rows[k] = load_vec<T, VEC>(ur + (k0 + k) * a.u_ts);
 #pragma unroll
         for (int k = 0; k < CONV_GROUP; ++k) {
-            if (!whole.value && tg + k >= tv) break;
+            if (!whole.value && t0 + k0 + k >= tv) break;
             Vec<T, VEC> o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
@@ -88,19 +99,21 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
                 float s = bias[i];
 #pragma unroll
                 for (int j = 0; j < W; ++j) s += w[j][i] * win[j][i];
-                o.v[i] = (T)(a.silu ? s * sigmoid(s) : s);
+                o.v[i] = (T)(silu.value ? s * sigmoid(s) : s);
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
             }
-            store_vec(yb + (long long)(tg + k) * a.D, o);
+            store_vec(yr + (long long)(k0 + k) * a.D, o);
         }
     };
-    if (tv == t0 + CONV_TR) {
+    either(a.silu, [&](auto silu) {
+        if (tv == t0 + CONV_TR) {
 #pragma unroll
-        for (int k = 0; k < CONV_TR; k += CONV_GROUP) group(t0 + k, std::true_type{});
-    } else {
-        for (int tg = t0; tg < tv; tg += CONV_GROUP) group(tg, std::false_type{});
-    }
+            for (int k = 0; k < CONV_TR; k += CONV_GROUP) group(k, std::true_type{}, silu);
+        } else {
+            for (int k = 0; t0 + k < tv; k += CONV_GROUP) group(k, std::false_type{}, silu);
+        }
+    });
     Vec<T, VEC> zero;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) zero.v[i] = (T)0.f;
@@ -114,7 +127,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs a) {
 
 // ds of step t and the step's row of u; `win` holds the W-1 rows before it and is shifted
 template <typename T, int W, int VEC>
-__device__ __forceinline__ void conv_slope(int silu, const Vec<T, VEC>& r, const Vec<T, VEC>& g, const float (&w)[W][VEC],
+__device__ __forceinline__ void conv_slope(bool silu, const Vec<T, VEC>& r, const Vec<T, VEC>& g, const float (&w)[W][VEC],
                                            const float (&bias)[VEC], float (&win)[W][VEC], float (&ds)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -140,7 +153,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
     const int cv = cb * a.cvb + tid % a.cvb;
     const long long row = (long long)rb * rows + tid / a.cvb;
     const int c = cv * VEC;
-    const int b = (int)(row / a.nch), t0 = (int)(row % a.nch) * CONV_TR;
+    const int b = (int)(row / a.nch), t0 = (int)(row % a.nch) * CONV_TR_BWD;
     float dw[W + 1][VEC];
 #pragma unroll
     for (int j = 0; j <= W; ++j)
@@ -162,7 +175,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
             for (int j = 0; j < W; ++j) ds[j][i] = 0.f;
         }
-        const int t1 = min(t0 + CONV_TR, a.L), tv = min(t1, len);
+        const int t1 = min(t0 + CONV_TR_BWD, a.L), tv = min(t1, len);
         if (t0 < tv) {
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) {
@@ -173,17 +186,24 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
         }
         // row k of the line's gradient is complete once ds of steps k-W+1 .. k is known
         const int tl = min(tv + W - 1, len);           // steps that are read
+        // the run's rows, one after the other: sums instead of products of 64 bits in every lane and access
+        const T* ur = ub + t0 * a.u_ts;
+        const T* gr = gb + t0 * a.dy_ts;
+        T* dr = db + (long long)t0 * a.D;
         // step k of the run; whole: all W - 1 steps behind the run are inside the sequence, so that only k decides
-        auto step = [&](int k, const Vec<T, VEC>& ru, const Vec<T, VEC>& rg, auto whole) {
+        auto step = [&](int k, const Vec<T, VEC>& ru, const Vec<T, VEC>& rg, auto whole, auto silu) {
             const int t = t0 + k;
             if (whole.value || t < tl) {
-                conv_slope<T, W, VEC>(a.silu, ru, rg, w, bias, win, ds[W - 1]);
-                if (whole.value ? k < CONV_TR : t < tv) {
+                conv_slope<T, W, VEC>(silu.value, ru, rg, w, bias, win, ds[W - 1]);
+                if (whole.value ? k < CONV_TR_BWD : t < tv) {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) dw[j][i] += ds[W - 1][i] * win[j][i];
                         dw[W][i] += ds[W - 1][i];
+                        // (added here: put off to the end, they would keep every step's ds and win in registers)
+#pragma unroll
+                        for (int j = 0; j <= W; ++j) asm volatile("" : "+v"(dw[j][i]));
                     }
                 }
 #pragma unroll
@@ -205,42 +225,49 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs a) {
                     for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * ds[j][i];
                     o.v[i] = (T)v;
                 }
-                store_vec(db + (long long)(t - (W - 1)) * a.D, o);
+                store_vec(dr, o);
+                dr += a.D;
             }
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) ds[j][i] = ds[j + 1][i];
         };
-        if (tv == t0 + CONV_TR && tl == tv + W - 1) {
-            constexpr int STEPS = CONV_TR + W - 1;
-            Vec<T, VEC> ru[2][CONV_GROUP], rg[2][CONV_GROUP];      // the next group's rows are loaded while this one's are used
-            auto fetch = [&](int g) {
+        either(a.silu, [&](auto silu) {
+            if (tv == t0 + CONV_TR_BWD && tl == tv + W - 1) {
+                constexpr int STEPS = CONV_TR_BWD + W - 1;
+                Vec<T, VEC> ru[2][CONV_GROUP], rg[2][CONV_GROUP];      // the next group's rows are loaded while this one's are used
+                auto fetch = [&](int g) {
 #pragma unroll
-                for (int k = 0; k < CONV_GROUP; ++k)
-                    if (g * CONV_GROUP + k < STEPS) {
-                        ru[g & 1][k] = load_vec<T, VEC>(ub + (t0 + g * CONV_GROUP + k) * a.u_ts);
-                        rg[g & 1][k] = load_vec<T, VEC>(gb + (t0 + g * CONV_GROUP + k) * a.dy_ts);
-                    }
-            };
-            fetch(0);
+                    for (int k = 0; k < CONV_GROUP; ++k)
+                        if (g * CONV_GROUP + k < STEPS) {
+                            ru[g & 1][k] = load_vec<T, VEC>(ur);
+                            rg[g & 1][k] = load_vec<T, VEC>(gr);
+                            ur += a.u_ts;
+                            gr += a.dy_ts;
+                        }
+                };
+                fetch(0);
 #pragma unroll
-            for (int g = 0; g * CONV_GROUP < STEPS; ++g) {
-                if ((g + 1) * CONV_GROUP < STEPS) fetch(g + 1);
+                for (int g = 0; g * CONV_GROUP < STEPS; ++g) {
+                    if ((g + 1) * CONV_GROUP < STEPS) fetch(g + 1);
 #pragma unroll
-                for (int k = 0; k < CONV_GROUP; ++k)
-                    if (g * CONV_GROUP + k < STEPS) step(g * CONV_GROUP + k, ru[g & 1][k], rg[g & 1][k], std::true_type{});
-            }
-        } else {
-            for (int t = t0; t < tv + W - 1; ++t) {
-                Vec<T, VEC> ru, rg;
-                if (t < tl) {
-                    ru = load_vec<T, VEC>(ub + t * a.u_ts);
-                    rg = load_vec<T, VEC>(gb + t * a.dy_ts);
+                    for (int k = 0; k < CONV_GROUP; ++k)
+                        if (g * CONV_GROUP + k < STEPS) step(g * CONV_GROUP + k, ru[g & 1][k], rg[g & 1][k], std::true_type{}, silu);
                 }
-                step(t - t0, ru, rg, std::false_type{});
+            } else {
+                for (int k = 0; t0 + k < tv + W - 1; ++k) {
+                    Vec<T, VEC> ru, rg;
+                    if (t0 + k < tl) {
+                        ru = load_vec<T, VEC>(ur);
+                        rg = load_vec<T, VEC>(gr);
+                        ur += a.u_ts;
+                        gr += a.dy_ts;
+                    }
+                    step(k, ru, rg, std::false_type{}, silu);
+                }
             }
-        }
+        });
         Vec<T, VEC> zero;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) zero.v[i] = (T)0.f;
@@ -338,7 +365,7 @@ inline int conv_cvb(int ncv) {
     while (v < ncv && v < 32) v *= 2;
     return v;
 }
-inline int conv_nch(int L) { return L > CONV_TR ? (L + CONV_TR - 1) / CONV_TR : 1; }
+inline int conv_nch(int L, int run) { return L > run ? (L + run - 1) / run : 1; }
 
 #define NMPC_W_SWITCH(W, ...)                                                                                      \
     switch (W) {                                                                                                   \
@@ -354,7 +381,7 @@ static int conv_check(const char* what, int nb, int L, int D, int W, int act) {
     NMPC_REQUIRE(W >= 1 && W <= CONV_MAX_W, "%s: %d taps (1..%d)", what, W, CONV_MAX_W);
     NMPC_REQUIRE(act == NMPC_ACT_NONE || act == NMPC_ACT_SILU, "%s: activation %d (none or silu)", what, act);
     NMPC_REQUIRE(L <= 1 << 30, "%s: at most 2^30 steps", what);
-    NMPC_REQUIRE((long long)nb * conv_nch(L) * D < (1ll << 31), "%s: too many elements for one launch", what);
+    NMPC_REQUIRE((long long)nb * conv_nch(L, CONV_TR) * D < (1ll << 31), "%s: too many elements for one launch", what);
     return 0;
 }
 
@@ -369,7 +396,7 @@ extern "C" int nmpc_causal_conv(int dtype, int nb, int L, int D, int W, const vo
     if (nb == 0) return 0;
     NMPC_REQUIRE(w && (L == 0 || (u && y)), "nmpc_causal_conv: null argument");
     ConvArgs a = {};
-    a.nb = nb; a.L = L; a.D = D; a.silu = act == NMPC_ACT_SILU; a.nch = conv_nch(L);
+    a.nb = nb; a.L = L; a.D = D; a.silu = act == NMPC_ACT_SILU; a.nch = conv_nch(L, CONV_TR);
     a.u = u; a.u_bs = u_bs; a.u_ts = u_ts; a.w = w; a.bias = bias; a.start = start; a.lengths = lengths;
     a.y = y; a.window = W > 1 ? window : nullptr;
     NMPC_DTYPE_SWITCH(dtype, {
@@ -390,7 +417,7 @@ extern "C" int nmpc_causal_conv(int dtype, int nb, int L, int D, int W, const vo
 extern "C" unsigned long long nmpc_causal_conv_workspace_bytes(int nb, int L, int D, int W) {
     if (nb <= 0 || L <= 0 || D <= 0 || W <= 0) return 0;
     // fewest runs a block can hold: 8, with 32 channel vectors
-    const unsigned long long nrb = ((unsigned long long)nb * conv_nch(L) + 7) / 8;
+    const unsigned long long nrb = ((unsigned long long)nb * conv_nch(L, CONV_TR_BWD) + 7) / 8;
     return nrb * (W + 1) * D * sizeof(float);
 }
 
@@ -404,7 +431,7 @@ extern "C" int nmpc_causal_conv_bwd(int dtype, int nb, int L, int D, int W, cons
                  workspace_bytes, nmpc_causal_conv_workspace_bytes(nb, L, D, W));
     NMPC_REQUIRE(workspace || nb == 0 || L == 0, "nmpc_causal_conv_bwd: null workspace");
     ConvArgs a = {};
-    a.nb = nb; a.L = L; a.D = D; a.silu = act == NMPC_ACT_SILU; a.nch = conv_nch(L);
+    a.nb = nb; a.L = L; a.D = D; a.silu = act == NMPC_ACT_SILU; a.nch = conv_nch(L, CONV_TR_BWD);
     a.u = u; a.u_bs = u_bs; a.u_ts = u_ts; a.w = w; a.bias = bias; a.start = start; a.lengths = lengths;
     a.dy = dy; a.dy_bs = dy_bs; a.dy_ts = dy_ts; a.dwindow = W > 1 ? dwindow : nullptr; a.du = du; a.dstart = W > 1 ? dstart : nullptr;
     a.part = (float*)workspace;

@@ -6,8 +6,10 @@
 // times as much).  Products run on the matrix cores with fp32 accumulation; dG and dU are rounded to the element type once, as
 // operands of the next products, which take both side by side: dx is one product over 2 F, [dWg; dWu] one of 2 F rows.
 // What bounds it: many rows the matrix cores, few rows reading the weights, a prompt of a few hundred rows the latency of its loads.
-// Measured: bf16 4096 x 2048 x 8192 forward 264 us (1.04 PFLOP/s), 305 with both projections kept, gradient 580 us: 0.95 over a training
-// step (the library's plain products of these sizes reach 1.1 .. 1.3); fp32 4096 x 256 x 1024 training 160 us (81 TFLOP/s); bf16 1 x 2048 x 8192 12.9 us, 5.2 TB/s.
+// Measured: bf16 4096 x 2048 x 8192 forward 264 us (1.04 PFLOP/s), 340 with both projections kept, gradient 585 us: 0.9 PFLOP/s over
+// training steps, which hold the chip at its power limit (the library's plain products of these sizes reach 1.1 .. 1.3; writing the
+// projections past the caches is 36 us faster alone and no faster in training steps); fp32 4096 x 256 x 1024 training 160 us
+// (81 TFLOP/s); bf16 1 x 2048 x 8192 12.9 us, 5.2 TB/s.
 #include <cmath>
 
 #include "seq_common.h"
@@ -49,7 +51,6 @@ struct NtArgs {
     float* part;                       // fp32 partial products [splits][M][N] instead of out
     int splits;
     int mt, nt;                        // tiles
-    int past_cache;                    // `pre` is larger than the last-level cache: written without staying there (wide only)
     int wide;                          // results may be stored in pieces of 16 bytes: rows of whole groups of eight, aligned
 };
 
@@ -306,13 +307,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[e] = activation(g.act, v[0][e]).x * v[1][e];
                 store8((T*)g.out + o, h, g.N - n, wide);
-                if (g.pre && g.past_cache) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4)
-                            if (n < g.N) __builtin_nontemporal_store(f32x4{v[c][e], v[c][e + 1], v[c][e + 2], v[c][e + 3]}, (f32x4*)(g.pre + c * (long long)g.M * g.N + o + e));
-                } else if (g.pre) {
+                if (g.pre) {
                     store8(g.pre + o, v[0], g.N - n, wide);
                     store8(g.pre + (long long)g.M * g.N + o, v[1], g.N - n, wide);
                 }
@@ -493,7 +488,7 @@ __global__ __launch_bounds__(256) void zero_kernel(T* p, long long n) {
     for (long long o = (long long)blockIdx.x * 256 + threadIdx.x; o < n; o += 256ll * gridDim.x) p[o] = (T)0.f;
 }
 
-// dG, dU from the saved projections (read once, past the cache that keeps the rows for the products): rows [Mp][2 Fp], dG then dU, zero past M and past F.  Bound by memory (2 e + 2 e + 8 + e bytes an
+// dG, dU from the saved projections: rows [Mp][2 Fp], dG then dU, zero past M and past F.  Bound by memory (2 e + 2 e + 8 + e bytes an
 // element): eight elements a thread; VEC: rows of pre and dh may be read in pieces of 16 bytes.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void gate_slope_kernel(int M, int F, int Mp, int Fp, int act, const float* pre, const T* dh, long long dh_ld, T* rows) {
@@ -509,8 +504,8 @@ __global__ __launch_bounds__(256) void gate_slope_kernel(int M, int F, int Mp, i
     if ((int)m < M) {
         if constexpr (VEC) {
             if (f < F) {               // F is a multiple of 8
-                *(f32x4*)g = __builtin_nontemporal_load((const f32x4*)(pre + o)); *(f32x4*)(g + 4) = __builtin_nontemporal_load((const f32x4*)(pre + o + 4));
-                *(f32x4*)u = __builtin_nontemporal_load((const f32x4*)(pre + total + o)); *(f32x4*)(u + 4) = __builtin_nontemporal_load((const f32x4*)(pre + total + o + 4));
+                *(float4*)g = *(const float4*)(pre + o); *(float4*)(g + 4) = *(const float4*)(pre + o + 4);
+                *(float4*)u = *(const float4*)(pre + total + o); *(float4*)(u + 4) = *(const float4*)(pre + total + o + 4);
 #pragma unroll
                 for (int i = 0; i < 8; i += E) *(Vec<T, E>*)(d + i) = load_vec<T, E>(dh + (long long)m * dh_ld + f + i);
             }
@@ -627,8 +622,6 @@ static int run_product(NtArgs g, hipStream_t st) {
     g.splits = shape.splits;
     if (g.splits == 1) g.part = nullptr;
     g.wide = g.N % 8 == 0 && ((uintptr_t)g.out | (uintptr_t)g.out1 | (uintptr_t)g.pre) % 16 == 0;
-    // 268 MB of projections (4096 x 2048 x 8192): 304 instead of 340 us; 134 MB (4096 x 1024 x 4096): 134 instead of 104
-    g.past_cache = GATED && g.wide && g.pre && 8ll * g.M * g.N > (192ll << 20);
     const int bn = GATED ? shape.bn / 2 : shape.bn;
     g.mt = (g.M + shape.bm - 1) / shape.bm;
     g.nt = (g.N + bn - 1) / bn;

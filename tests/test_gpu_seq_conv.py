@@ -74,6 +74,13 @@ def test_forward_and_gradients(nb, steps, d, taps, dtype, act, bias, start, leng
         assert (grads[k] is None) == (k not in named), k
 
 
+@pytest.mark.parametrize("steps", [15, 17, 27, 28, 29, 31, 32, 55, 56, 57, 59, 85])
+@pytest.mark.parametrize("act,cut", [("silu", 0), (None, 9)])
+def test_ends_of_runs(steps, act, cut):
+    """Either side of the runs of steps that a thread owns, forward (16) and backward (28)."""
+    test_forward_and_gradients(2, steps, 20, 4, "f32", act, True, True, [steps, steps - cut])
+
+
 def test_no_sequences():
     y, window, saved = nmpc_amd.causal_conv_fwd(torch.zeros(0, 5, 8, device="cuda"), torch.ones(8, 3, device="cuda"), torch.ones(8, device="cuda"))
     grads = nmpc_amd.causal_conv_bwd(saved, torch.zeros(0, 5, 8, device="cuda"))

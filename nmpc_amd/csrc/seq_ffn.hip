@@ -275,8 +275,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(NtArgs g) {
     // at piece ^ (row & 15) against bank conflicts.
     constexpr int PER = (BM + BN) * 64 / 8192;
     static_assert(4 * PER >= WAVES, "room for the results");
-    const int place = wave / PER;
-    float* stage = reinterpret_cast<float*>(place == 0 ? lds0 : place == 1 ? lds1 : place == 2 ? lds2 : lds3) + (wave % PER) * 2048;
+    float* stage = reinterpret_cast<float*>(wave < PER ? lds0 : 2 * PER >= WAVES || wave < 2 * PER ? lds1 : wave < 3 * PER ? lds2 : lds3) + (wave % PER) * 2048;
     const bool wide = g.wide;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -556,7 +555,7 @@ static bool tiled(const void* p, long long ld, int K, bool by_k) {
 // Tile size and splits of a product: the choice of least estimated time.  A 256 x 256 tile has a CU for itself, two 128 x 128 tiles share
 // one; a k-tile of the large one takes 1.06 us in 16 bits and 4.0 us in fp32 (measured at 16384 x 2048 x 4096), of the small one a
 // quarter of it and a sixth more, less well used where a CU has one alone.  Tiles of 64 x 128 (`small`: A's rows lie along k) divide few
-// rows more finely and cost 0.24 and 0.56 us a k-tile: 512 x 2048 x 2048 in bf16 19 instead of 24 us, 256 x 1024 x 4096 in fp32 42 instead
+// rows more finely and cost 0.24 and 0.60 us a k-tile: 512 x 2048 x 2048 in bf16 19 instead of 24 us, 256 x 1024 x 4096 in fp32 42 instead
 // of 71; at 1024 x 1024 x 4096 they take 37 instead of 29 and 142 instead of 139.  Every round of tiles pays for filling and draining;
 // a split contraction pays for writing and reading its partial products.
 struct Shape {
@@ -575,7 +574,7 @@ static Shape product_shape(int M, int N, int ktiles, bool small, bool may_split)
             double t;
             if (tile == 2) t = ceil(n / 256) * (depth * ktime + fill);
             else if (tile == 1) t = n <= 256 ? depth * ktime * 0.25 * (sizeof(T) == 2 ? 1.25 : 1.0) + fill : ceil(n / 512) * (depth * ktime * 0.5 * 1.17 + fill);
-            else t = ceil(n / 256) * depth * (sizeof(T) == 2 ? 0.24 : 0.56) + fill;
+            else t = ceil(n / 256) * depth * (sizeof(T) == 2 ? 0.24 : 0.60) + fill;
             if (splits > 1) t += 6.0 + (double)splits * M * N * 8 / 4.5e6;
             if (t < best.us) best = {bm, bn, splits, t};
         }

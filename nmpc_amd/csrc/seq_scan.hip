@@ -46,8 +46,11 @@ __device__ __forceinline__ float softplus(float x) {
     return fmaxf(x, 0.f) + 2.f * s * r;
 }
 
-// What many steps do to a state, 2^x: an unstable mode's growth over them stays finite, so that a state of zero stays zero.
-__device__ __forceinline__ float decay_of(float x) { return fminf(__builtin_amdgcn_exp2f(x), 3.4e38f); }
+// What many steps do to a state: x 2^e, as three products with 2^(e/3).  A growing mode may grow past any fp32 number on a state so small
+// that the result is an ordinary one, or on a state of zero: each factor stays at or below 2^127, and all three carry the smallest number
+// past the largest, so that nothing but the result's own overflow is lost.  One factor, which cannot do that, would save 1 .. 2 % of the
+// slots kernel (4 x 2048 x 2048, 16 states: 126 instead of 128 us).
+__device__ __forceinline__ float growth_root(float e) { return __builtin_amdgcn_exp2f(fminf(e * (1.f / 3.f), 127.f)); }
 
 template <int CTRL, int BANKS = 0xf>
 __device__ __forceinline__ float dpp(float v) {
@@ -473,21 +476,21 @@ __global__ __launch_bounds__(SCAN_THREADS, P == 1 ? 1 : 2) void scan_slots_kerne
         float (*end)[64][8] = ends[tile & 1];
         store_four(end[w][lane], x);
         {
-            float decay[4];
+            float root[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) decay[i] = decay_of(total_d * A[i]);
-            store_four(end[w][lane] + 4, decay);
+            for (int i = 0; i < 4; ++i) root[i] = growth_root(total_d * A[i]);
+            store_four(end[w][lane] + 4, root);
         }
         __syncthreads();                              // (the other half of `ends` is free again: everyone is past its reads)
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
-            float xe[4], de[4];
+            float xe[4], root[4];
             load_four(end[k][lane], xe);
-            load_four(end[k][lane] + 4, de);
+            load_four(end[k][lane] + 4, root);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = k == w ? carry[i] : x[i];
-                carry[i] = de[i] * carry[i] + xe[i];
+                carry[i] = root[i] * (root[i] * (root[i] * carry[i])) + xe[i];
             }
         }
         if (a.saved && ok && t0 < a.L)
@@ -552,7 +555,8 @@ __global__ __launch_bounds__(256) void scan_chunks_kernel(ScanDev s, int NP) {
         float* p = s.xin + (at * a.D + ch) * NP + n;
         const float own = *p;
         *p = x;
-        x = decay_of(A * s.dsum[at * a.D + ch]) * x + own;
+        const float root = growth_root(A * s.dsum[at * a.D + ch]);
+        x = root * (root * (root * x)) + own;
     }
 }
 

@@ -348,3 +348,44 @@ def test_autograd_is_the_pair_and_capture():
         torch.cuda.synchronize()
         for a, e in zip(outs, step()):
             assert torch.equal(a, e)
+
+
+GROWTH_CASES = [  # nb, steps, d, bits a step, size of the states and of the adjoints
+    (2, 40, 8, 8.6, 1e-30),           # the time axis in slots of 16 steps, the gradient whole
+    (1, 600, 8, 8.6, 1e-30),          # in parts of 32 steps, both passes
+    (2, 1100, 24, 8.6, 1e-30),
+    (120, 40, 1000, 8.6, 1e-30),      # whole sequences
+    (2, 40, 8, 15.2, 2.0 ** -126),    # growth past the square root of 2^253, from the smallest normal number
+    (1, 600, 8, 15.2, 2.0 ** -126),
+]
+
+
+@pytest.mark.parametrize("nb,steps,d,bits,size", GROWTH_CASES)
+def test_growing_modes_of_small_states(nb, steps, d, bits, size):
+    """Sixteen steps multiply a state, and the adjoint of one, by 2^138 or 2^243: more than a number of fp32 holds, on states so small that
+    the results are ordinary numbers.  The steps around them leave a state as it is, so that later parts see what earlier ones did."""
+    v, dy, dlast = _inputs(steps, nb, steps, d, 4, 1, "f32", skip=False, gate=False, bias=False)
+    growth = bits * 0.6931471805599453
+    v["A"] = growth * torch.tensor([1.0, 0.5, -0.01, -1.0]).expand(d, 4).contiguous()
+    v["dt"] = torch.zeros_like(v["dt"])
+    v["dt"][:, 16:32] = 1.0
+    # signs and powers of two: whole parts of the range are left for the growth
+    v["start"] = torch.sign(v["start"]) * size
+    v["u"], dy, dlast = torch.zeros_like(v["u"]), torch.zeros_like(dy), torch.sign(dlast) * size
+    want_y, want_last = oracle.lpv_scan(*[f64(v[k]) for k in NAMES[:8]], use_softplus=False, start=f64(v["start"]))
+    y, last, saved = nmpc_amd.lpv_scan_fwd(*[gpu(v[k]) for k in NAMES[:8]], False, gpu(v["start"]))
+    m = _magnitudes(v, dy, dlast, False, None)
+    # the exponent of a step is rounded twice (A log2 e, its product with delta), of a part likewise: 2 roundings a unit of the
+    # exponent of all sixteen steps; two more a step (exponential, product), three factors of two roundings where parts are joined
+    r = 52 + 4 + 2 * 16 * growth + 2 * 16 + 6 * 3
+    tiny = 2.0 ** -126                 # decaying states may round to multiples of 2^-149, or to zero
+    assert_close(last, want_last, r, m["last"], "last", tiny)
+    assert_close(y, want_y, r, m["y"], "y", 8 * tiny)
+    got = nmpc_amd.lpv_scan_bwd(saved, gpu(dy), gpu(dlast))
+    # the adjoint of the state before the first step: the same factors from behind
+    decay = torch.exp(16 * f64(v["A"]))[None]
+    assert_close(got["dstart"], decay * f64(dlast), r, decay * f64(dlast).abs(), "dstart", tiny)
+    # as stepwise: what leaves the range of fp32 does so in every plan
+    v["A"][:, 0] = 40.0
+    over = nmpc_amd.lpv_scan_fwd(*[gpu(v[k]) for k in NAMES[:8]], False, gpu(v["start"]))[1]
+    assert torch.isinf(over[..., 0]).all() and torch.equal(torch.sign(over[..., 0]).cpu(), torch.sign(v["start"][..., 0]))

@@ -3,7 +3,8 @@
 Each whole-sequence operator comes in three forms: `op(...)` (differentiable through torch.autograd where an input asks for
 it), and the pair `op_fwd(...)` -> outputs and what the gradient needs, `op_bwd(saved, gradients of the outputs)` -> the
 gradients, which records no autograd graph and can be captured into a HIP graph.  `*_step` is the form for one sample of
-every running sequence and moves its state on in place.
+every running sequence and moves its state on in place.  Derivatives are first order and reverse mode: tensors that carry a
+forward-mode tangent are refused.
 
 Samples are [batch, steps, channels] (channels contiguous; other layouts are copied) in float32, bfloat16 or float16;
 states of the scan and all sums are fp32.  `lengths` [batch] (integers, on the GPU): steps from lengths[b] on are padding -
@@ -11,6 +12,7 @@ they are not read, and their outputs and gradients are zero."""
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import NmpcError, lib
@@ -94,9 +96,19 @@ def _lengths(what, t, nb):
     return t.to(torch.int32).contiguous()
 
 
+def _no_tangents(what, *tensors):
+    """Refuses tensors that carry a forward-mode tangent, which the kernels would drop: there is no form that computes one."""
+    if getattr(forward_ad, "_current_level", 0) < 0:           # no forward-mode level is open: nothing to look for
+        return
+    for t in tensors:
+        if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            _fail(what, "has no forward-mode derivative, and an input carries a tangent")
+
+
 def _records(what, *tensors):
     """Does this call have to be recorded by autograd?  Under graph capture it is refused: autograd's own bookkeeping of
     leaves that an eager graph still holds cannot be captured."""
+    _no_tangents(what, *tensors)
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
@@ -175,6 +187,7 @@ def _conv_fwd(what, u, w, bias, act, start, lengths, want_window):
 
 def causal_conv_fwd(u, w, bias=None, act=None, start=None, lengths=None):
     """causal_conv that keeps what its gradient needs: (y, window, saved)."""
+    _no_tangents("causal_conv_fwd", u, w, bias, start)
     y, window, tensors = _conv_fwd("causal_conv_fwd", u, w, bias, act, start, lengths, True)
     return y, window, Saved("causal_conv", tensors, (act,))
 
@@ -183,6 +196,7 @@ def causal_conv_bwd(saved, dy, dwindow=None):
     """Gradients of causal_conv_fwd's call: {"du", "dw", "dbias", "dstart"} (dw and dbias fp32; None for inputs that were
     not given).  dy [batch, steps, channels] and dwindow [batch, taps-1, channels] (None = zero): gradients of y and window."""
     what = "causal_conv_bwd"
+    _no_tangents(what, dy, dwindow)
     (u, w, bias, start, lengths), (act,) = _saved("causal_conv", saved)
     nb, steps, d = u.shape
     taps = w.shape[1]
@@ -327,6 +341,7 @@ def _scan_fwd(what, u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, wan
 def lpv_scan_fwd(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, start=None, lengths=None):
     """lpv_scan that keeps what its gradient needs: (y, last, saved).  Besides the inputs that is the state before every
     16th step."""
+    _no_tangents("lpv_scan_fwd", u, dt, A, B, C, D, z, dt_bias, start)
     y, last, tensors = _scan_fwd("lpv_scan_fwd", u, dt, A, B, C, D, z, dt_bias, softplus, start, lengths, True, True)
     return y, last, Saved("lpv_scan", tensors, (bool(softplus),))
 
@@ -336,6 +351,7 @@ def lpv_scan_bwd(saved, dy, dlast=None):
     in the samples' type, the others fp32; None for inputs that were not given.  dy [batch, steps, channels] and dlast
     [batch, channels, states] (None = zero): gradients of y and of the last state."""
     what = "lpv_scan_bwd"
+    _no_tangents(what, dy, dlast)
     (u, dt, A, B, C, D, z, dt_bias, start, lengths, kept), (softplus,) = _saved("lpv_scan", saved)
     dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
     dlast = _states(what, "dlast", dlast, u.shape[0], A)
@@ -434,6 +450,7 @@ def _ffn_fwd(what, x, w_gate, w_up, act, want_saved):
 
 def gated_ffn_fwd(x, w_gate, w_up, act="silu"):
     """gated_ffn that keeps what its gradient needs: (h, saved).  Besides the inputs that is both projections in fp32."""
+    _no_tangents("gated_ffn_fwd", x, w_gate, w_up)
     h, tensors = _ffn_fwd("gated_ffn_fwd", x, w_gate, w_up, act, True)
     return h, Saved("gated_ffn", tensors, (act, tuple(x.shape)))
 
@@ -441,6 +458,7 @@ def gated_ffn_fwd(x, w_gate, w_up, act="silu"):
 def gated_ffn_bwd(saved, dh):
     """Gradients (dx, dw_gate, dw_up) of gated_ffn_fwd's call, in the inputs' type; dh like h."""
     what = "gated_ffn_bwd"
+    _no_tangents(what, dh)
     (rows, w_gate, w_up, pre), (act, shape) = _saved("gated_ffn", saved)
     (m, k), f = rows.shape, w_gate.shape[0]
     dh = _samples(what, "dh", dh, shape[:-1] + (f,), rows.dtype).reshape(m, f)

@@ -193,3 +193,33 @@ def test_ffn_abi_refusals():
     assert rc != 0 and b"workspace" in L.nmpc_last_error()
     rc = L.nmpc_gated_ffn_bwd(1, 100, 64, 128, p, 64, p, 64, p, 64, 1, None, p, 128, p, p, p, p, need, None)
     assert rc != 0 and b"null" in L.nmpc_last_error()
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor does not ask for a gradient, and its tangent would be dropped: every form refuses it, with gradients enabled or not."""
+    from torch.autograd import forward_ad
+    u, w, A, B, x, wg = torch.zeros(2, 6, 8), torch.zeros(8, 4), torch.zeros(8, 4), torch.zeros(2, 6, 2, 4), torch.zeros(3, 8), torch.zeros(6, 8)
+    scan = dict(u=u, dt=u, A=A, B=B, C=B, D=torch.zeros(8), z=u, dt_bias=torch.zeros(8), start=torch.zeros(2, 8, 4))
+    one = {k: t[:, 0] if k in ("u", "dt", "B", "C", "z") else t for k, t in scan.items() if k != "start"}
+    one["state"] = scan["start"]
+    conv = dict(u=u, w=w, bias=torch.zeros(8), start=torch.zeros(2, 3, 8))
+    step = dict(window=torch.zeros(2, 3, 8), u=u[:, 0], w=w, bias=torch.zeros(8))
+    ffn = dict(x=x, w_gate=wg, w_up=wg)
+    calls = [(nmpc_amd.causal_conv, conv), (nmpc_amd.causal_conv_fwd, conv), (nmpc_amd.causal_conv_step, step), (nmpc_amd.lpv_scan, scan),
+             (nmpc_amd.lpv_scan_fwd, scan), (nmpc_amd.lpv_scan_step, one), (nmpc_amd.gated_ffn, ffn), (nmpc_amd.gated_ffn_fwd, ffn)]
+    with forward_ad.dual_level():
+        for fn, args in calls:
+            for name in args:
+                dual = {**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))}
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(nmpc_amd.NmpcError, match="tangent"):
+                        fn(**dual)
+        for fn, grads in ((nmpc_amd.causal_conv_bwd, ("dy", "dwindow")), (nmpc_amd.lpv_scan_bwd, ("dy", "dlast")), (nmpc_amd.gated_ffn_bwd, ("dh",))):
+            for name in grads:
+                with pytest.raises(nmpc_amd.NmpcError, match="tangent"):
+                    fn(None, **{**dict.fromkeys(grads, u), name: forward_ad.make_dual(u, u)})
+        with pytest.raises(nmpc_amd.NmpcError) as plain:                # a level is open, but nothing carries a tangent
+            nmpc_amd.gated_ffn(x.double(), wg, wg)
+    assert "tangent" not in str(plain.value)
+    with pytest.raises(nmpc_amd.NmpcError, match="tangent"):
+        torch.func.jvp(lambda v: nmpc_amd.gated_ffn(v, wg, wg), (x,), (x,))

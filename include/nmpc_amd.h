@@ -327,6 +327,9 @@ typedef struct nmpc_scan_args {
 } nmpc_scan_args;
 unsigned long long nmpc_lpv_scan_saved_bytes(int nb, int L, int D, int N);
 unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D, int N, int G, int backward);
+/* How a pass of this size runs: 1 = whole sequences one step after the other, n > 1 = in n parts of the time axis side by side,
+ * 0 = in slots of a workgroup; -1 for sizes that no call has. */
+int nmpc_lpv_scan_plan(int nb, int L, int D, int N, int G, int backward);
 int nmpc_lpv_scan(const nmpc_scan_args* args, void* stream);
 int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream);
 int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream);
@@ -339,6 +342,9 @@ int nmpc_lpv_scan_step(const nmpc_scan_args* args, void* stream);
  * calls that overlap in time need one each.  dG and dU (dh times the other factor and the slope) are rounded to the element
  * type once, as operands of the gradients' products: in fp16 they have that type's range. */
 unsigned long long nmpc_gated_ffn_workspace_bytes(int dtype, int M, int K, int F, int backward, int copy);
+/* Which kernel a product takes (0 = forward, 1 = dx, 2 = the weights' gradients): rows and columns of its tiles and the parts of its
+ * contraction; columns = 32 is the kernel for few rows. */
+int nmpc_gated_ffn_plan(int dtype, int M, int K, int F, int product, int copy, int shape[3]);
 int nmpc_gated_ffn(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld, const void* wu,
                    long long wu_ld, int act, void* h, float* pre, void* workspace, unsigned long long workspace_bytes, void* stream);
 int nmpc_gated_ffn_bwd(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld, const void* wu,

@@ -76,10 +76,12 @@ SIGNATURES = {
                                              ctypes.c_int, c_void_p, c_void_p]),
     "nmpc_lpv_scan_saved_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 4),
     "nmpc_lpv_scan_workspace_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 6),
+    "nmpc_lpv_scan_plan": (ctypes.c_int, [ctypes.c_int] * 6),
     "nmpc_lpv_scan": (ctypes.c_int, [c_void_p, c_void_p]),
     "nmpc_lpv_scan_bwd": (ctypes.c_int, [c_void_p, c_void_p]),
     "nmpc_lpv_scan_step": (ctypes.c_int, [c_void_p, c_void_p]),
     "nmpc_gated_ffn_workspace_bytes": (ctypes.c_ulonglong, [ctypes.c_int] * 6),
+    "nmpc_gated_ffn_plan": (ctypes.c_int, [ctypes.c_int] * 6 + [c_void_p]),
     "nmpc_gated_ffn": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p, ctypes.c_longlong] * 3 + [ctypes.c_int] + [c_void_p] * 3 +
                        [ctypes.c_ulonglong, c_void_p]),
     "nmpc_gated_ffn_bwd": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p, ctypes.c_longlong] * 3 + [ctypes.c_int, c_void_p, c_void_p,

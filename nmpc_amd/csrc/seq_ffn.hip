@@ -643,6 +643,18 @@ static unsigned pad_grid(long long total) {
     return (unsigned)(blocks < 8192 ? blocks : 8192);
 }
 
+// Which kernel a product takes: the forward pass (0), dx (1) or [dWg; dWu] (2).
+template <typename T>
+static Shape shape_of(int M, int K, int F, int product, bool copy) {
+    const int kt = ktile<T>(), Fp = up_to(F, kt), Mp = up_to(M, kt);
+    if (product == 1) return product_shape<T>(M, K, 2 * Fp / kt, true, true);
+    if (product == 2) return product_shape<T>(2 * Fp, K, Mp / kt, false, true);
+    const bool aligned = !copy && K % kt == 0;
+    if (!serves_few<T>(M, K, F, aligned)) return product_shape<T>(M, 2 * F, (K + kt - 1) / kt, true, false);
+    const FewShape fs = few_shape<T>(M, K, F, !copy && K % (16 / (int)sizeof(T)) == 0);
+    return {16 * fs.mb, 32, fs.waves, fs.us};
+}
+
 // The workspace of a call: copies of operands that cannot be read in pieces as they are, and the gradient's intermediates.
 struct FfnSpace {
     unsigned long long bytes, x, wg, wu, rows, part;
@@ -661,7 +673,7 @@ struct FfnSpace {
         }
         if (!backward) return s;
         s.rows = take(e * Mp * 2 * Fp);
-        const Shape a = product_shape<T>(M, K, 2 * Fp / kt, true, true), b = product_shape<T>(2 * Fp, K, Mp / kt, false, true);
+        const Shape a = shape_of<T>(M, K, F, 1, copy), b = shape_of<T>(M, K, F, 2, copy);
         const unsigned long long pa = a.splits > 1 ? 4ull * a.splits * M * K : 0, pb = b.splits > 1 ? 4ull * b.splits * 2 * Fp * K : 0;
         s.part = take(pa > pb ? pa : pb);
         return s;
@@ -753,6 +765,14 @@ extern "C" unsigned long long nmpc_gated_ffn_workspace_bytes(int dtype, int M, i
     if (M <= 0 || K <= 0 || F <= 0) return 0;
     return dtype == NMPC_F32 ? FfnSpace::plan<float>(M, K, F, backward != 0, copy != 0).bytes
                              : FfnSpace::plan<bf16>(M, K, F, backward != 0, copy != 0).bytes;
+}
+
+extern "C" int nmpc_gated_ffn_plan(int dtype, int M, int K, int F, int product, int copy, int shape[3]) {
+    if (ffn_check("nmpc_gated_ffn_plan", dtype, M, K, F, NMPC_ACT_SILU)) return 1;
+    NMPC_REQUIRE(M >= 1 && product >= 0 && product <= 2 && shape, "nmpc_gated_ffn_plan: bad argument");
+    const Shape s = dtype == NMPC_F32 ? shape_of<float>(M, K, F, product, copy != 0) : shape_of<bf16>(M, K, F, product, copy != 0);
+    shape[0] = s.bm; shape[1] = s.bn; shape[2] = s.splits;
+    return 0;
 }
 
 extern "C" int nmpc_gated_ffn(int dtype, int M, int K, int F, const void* x, long long x_ld, const void* wg, long long wg_ld,

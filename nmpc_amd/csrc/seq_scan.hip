@@ -1095,6 +1095,14 @@ extern "C" unsigned long long nmpc_lpv_scan_workspace_bytes(int nb, int L, int D
     return scan_workspace(s, backward != 0, nullptr);
 }
 
+extern "C" int nmpc_lpv_scan_plan(int nb, int L, int D, int N, int G, int backward) {
+    if (nb <= 0 || L <= 0 || L > 1 << 30 || D <= 0 || N <= 0 || N > 64 || G <= 0 || D % G) return -1;
+    ScanDev s = {};
+    s.a.nb = nb; s.a.L = L; s.a.D = D; s.a.N = N; s.a.G = G;
+    scan_plan(s, backward != 0);
+    return s.slots ? 0 : s.nch;
+}
+
 extern "C" int nmpc_lpv_scan(const nmpc_scan_args* args, void* stream) {
     if (scan_check("nmpc_lpv_scan", args)) return 1;
     ScanDev s = {};

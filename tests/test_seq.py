@@ -223,3 +223,22 @@ def test_forward_mode_tangents_are_refused():
     assert "tangent" not in str(plain.value)
     with pytest.raises(nmpc_amd.NmpcError, match="tangent"):
         torch.func.jvp(lambda v: nmpc_amd.gated_ffn(v, wg, wg), (x,), (x,))
+
+
+def test_plan_queries():
+    """Which kernels calls take: the refusals, and agreement with the workspaces."""
+    L = _lib.lib()
+    plan = L.nmpc_lpv_scan_plan
+    for bad in ((0, 4, 4, 4, 1), (1, 0, 4, 4, 1), (1, 4, 0, 4, 1), (1, 4, 4, 65, 1), (1, 4, 4, 4, 3), (1, 4, 4, 4, 0)):
+        assert plan(*bad, 0) == -1 and plan(*bad, 1) == -1
+    for size in ((1, 1, 1, 1, 1), (1, 8192, 2048, 16, 1), (4, 2048, 2048, 16, 1), (120, 40, 1000, 8, 2), (2, 400, 10, 49, 2)):
+        parts = plan(*size, 0)                        # parts have a workspace, the others none
+        assert parts >= 0 and (parts > 1) == (L.nmpc_lpv_scan_workspace_bytes(*size, 0) > 0), size
+        assert plan(*size, 1) >= 1, size
+    shape = (ctypes.c_int * 3)()
+    at = ctypes.addressof(shape)
+    for bad in ((3, 4, 4, 4, 0, 0, at), (0, 0, 4, 4, 0, 0, at), (0, 4, 0, 4, 0, 0, at), (0, 4, 4, 4, 3, 0, at), (0, 4, 4, 4, -1, 0, at), (0, 4, 4, 4, 0, 0, None)):
+        assert L.nmpc_gated_ffn_plan(*bad) != 0 and b"nmpc_gated_ffn_plan" in L.nmpc_last_error(), bad
+    for product, most in ((0, (64, 32, 16)), (1, (256, 256, 64)), (2, (256, 256, 64))):       # one row: the kernel for few rows forward
+        assert L.nmpc_gated_ffn_plan(1, 1, 2048, 8192, product, 0, at) == 0
+        assert all(1 <= v <= top for v, top in zip(shape, most)) and (shape[1] == 32) == (product == 0)

@@ -19,6 +19,7 @@
 // Measured, bf16, 16 states: 4 x 2048 steps x 2048 channels forward 122 us, training 483 us (279 of them the main backward pass);
 // 1 x 8192 x 2048 forward 152 us; step of 64 x 4096 channels 9.5 us, 3.8 TB/s.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "seq_common.h"
@@ -983,16 +984,24 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanDev s) {
 static int scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // How a pass runs: whole sequences one tile after the other, the time axis in slots of a workgroup (forward only), or in chunks with a
-// summary pass before; the least of three estimated times.  Each is the longer of the steps that follow one another and of the work at the
-// rate of a full chip (us a state and step; bf16, 16 states).  Measured, in us:                       whole   slots   chunks
-//   forward   1 x 8192 x 2048 channels (268 M states and steps)                                         1025     400      162
-//             2 x 2048 x 2048                                                                                    104       85
-//             4 x 2048 x 2048                                                                            262     122      143
-//             8 x 2048 x 2048                                                                                    221      275
-//             8 x 2048 x 4096                                                                            372     413      541
-//   backward  4 x 2048 x 2048                                                                            880              350
-//             fp32 64 x 50 x 64, 8 states, both passes called eagerly                                        58               64
-//             64 x 50 x 64 channels of 8 states, called eagerly                                             58               64
+// summary pass before; the least of the estimated times (us).  Each is made of the steps that follow one another and of the work at the rate
+// of a full chip (bf16, 16 states); chunks pay besides for two more launches, partial sums, and a join that goes through them one after the
+// other: few channels in as many chunks as fill the chip would spend their time there, so that longer ones are looked at too.
+// Measured, in us (16 states and bf16 unless noted; chunks of .. tiles):       whole   slots   chunks
+//   forward   1 x 8192 x 2048 channels (268 M states and steps)                 870     350    141 (8), 150 (16), 206 (1)
+//             1 x 8192 x 64                                                     870     350     85 (1),  49 (4),   64 (8)
+//             1 x 2000 x 512, 8 states                                          260     101     36 (1),  33 (2),   42 (4)
+//             2 x 2048 x 2048                                                   223      93     77 (4),  80 (8)
+//             4 x 2048 x 2048                                                   224     116    130 (4), 134 (8)
+//             8 x 2048 x 2048                                                   225     205    236 (4), 251 (16)
+//             16 x 512 x 2048                                                    84      97    127 (4)
+//   backward  1 x 8192 x 64                                                    3000            121 (1),  91 (2),   98 (4)
+//             4 x 2048 x 2048                                                   783            320 (4), 318 (8)
+//             16 x 512 x 2048                                                   252            316 (4), 362 (1)
+//             64 x 100 x 256                                                     60              77 (1)
+//             fp32, 64 sequences of 33 .. 64 steps, 32 .. 256 channels,
+//             8 or 16 states                                                  37..46          45..50 (1)
+//             the same of 100 steps, 32 .. 128 channels                       57..69          52..61 (1)
 static void scan_plan(ScanDev& s, bool backward) {
     const nmpc_scan_args& a = s.a;
     const int P = scan_lanes(a.N), CH = SCAN_THREADS / P;
@@ -1005,11 +1014,18 @@ static void scan_plan(ScanDev& s, bool backward) {
     const long long base = (long long)a.nb * a.G * s.nblk;
     if (base == 0 || s.ntile == 0) return;
     const double work = (double)a.nb * a.D * a.L * 4 * P * 1e-6;
-    const long long want = (1024 + base - 1) / base;            // chunks that fill the chip: four workgroups a CU
-    const int n = want < s.ntile ? (int)want : s.ntile, tpc = (s.ntile + n - 1) / n;
     const double whole = std::max((backward ? 13.7 : 4.0) * s.ntile, (backward ? 1.03 : 0.35) * work);
     const double slots = backward ? 1e30 : std::max(3.0 * ((a.L + 63) / 64), 0.45 * work);
-    const double chunks = n > 1 ? std::max((backward ? 17.0 : 6.6) * tpc, (backward ? 1.29 : 0.58) * work) + (backward ? 12.0 : 10.0) : 1e30;
+    const long long want = (1024 + base - 1) / base;            // chunks that fill the chip: four workgroups a CU
+    double chunks = 1e30;
+    int tpc = s.ntile;
+    for (long long t = want < s.ntile ? (s.ntile + want - 1) / want : 1; t < s.ntile; t *= 2) {
+        // the longer of both, and more where they are alike: workgroups that share a CU slow each other down
+        const double chain = (backward ? 14.3 : 5.6) * t, bulk = (backward ? 1.10 : 0.44) * work;
+        const double us = std::cbrt(chain * chain * chain + bulk * bulk * bulk) + (backward ? 24.0 : 10.0) +
+                          (backward ? 0.35 : 0.26) * (double)((s.ntile + t - 1) / t);
+        if (us < chunks) { chunks = us; tpc = (int)t; }
+    }
     if (slots < whole && slots <= chunks) {
         s.slots = 1;
     } else if (chunks < whole) {

@@ -84,6 +84,14 @@ def test_scan_in_parts(n, dtype):
     _check(v, dy, dlast, True, [steps, steps - 37])
 
 
+@pytest.mark.parametrize("steps,n", [(4000, 16), (4017, 5)])
+def test_scan_in_parts_of_several_tiles(steps, n):
+    """Few channels over many steps: parts of more than one tile, so that the join of them stays short."""
+    assert all(1 < _scan_plan(1, steps, 6, n, 1, b) < (steps + 31) // 32 for b in (0, 1))
+    v, dy, dlast = _scan_inputs(n, 1, steps, 6, n, 1, "f32")
+    _check(v, dy, dlast, True, [steps - 5])
+
+
 @pytest.mark.parametrize("n", [3, 8, 16, 24, 64])
 def test_scan_in_slots(n):
     nb, steps, d, groups = 2, 70, 10, 2

@@ -175,7 +175,8 @@ def _conv_fwd(what, u, w, bias, act, start, lengths, want_window):
     nb, steps, d = u.shape
     taps = w.shape[1]
     if start is not None:
-        start = _samples(what, "start", start, (nb, taps - 1, d), u.dtype).contiguous()
+        start = _samples(what, "start", start, (nb, taps - 1, d), u.dtype)
+        start = start if start.is_contiguous() else start.detach().contiguous()
     lengths = _lengths(what, lengths, nb)
     i = _on_gpu(what, u, w, bias, start, lengths)
     y = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
@@ -201,7 +202,7 @@ def causal_conv_bwd(saved, dy, dwindow=None):
     nb, steps, d = u.shape
     taps = w.shape[1]
     dy = torch.zeros_like(u) if dy is None else _samples(what, "dy", dy, u.shape, u.dtype)
-    dwindow = None if dwindow is None else _samples(what, "dwindow", dwindow, (nb, taps - 1, d), u.dtype).contiguous()
+    dwindow = None if dwindow is None else _samples(what, "dwindow", dwindow, (nb, taps - 1, d), u.dtype).detach().contiguous()
     i = _on_gpu(what, u, dy, dwindow)
     du = torch.empty((nb, steps, d), dtype=u.dtype, device=u.device)
     dw = torch.empty_like(w)
@@ -461,7 +462,7 @@ def gated_ffn_bwd(saved, dh):
     _no_tangents(what, dh)
     (rows, w_gate, w_up, pre), (act, shape) = _saved("gated_ffn", saved)
     (m, k), f = rows.shape, w_gate.shape[0]
-    dh = _samples(what, "dh", dh, shape[:-1] + (f,), rows.dtype).reshape(m, f)
+    dh = _samples(what, "dh", dh, shape[:-1] + (f,), rows.dtype).detach().reshape(m, f)
     i = _on_gpu(what, rows, dh)
     dx = torch.empty(shape, dtype=rows.dtype, device=rows.device)
     dwg, dwu = (torch.empty((f, k), dtype=rows.dtype, device=rows.device) for _ in range(2))

@@ -179,3 +179,24 @@ def test_other_stream():
         got = nmpc_amd.causal_conv(u.cuda(), w.cuda(), b.cuda(), "silu")
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_the_pair_records_nothing():
+    """Leaves that have to be copied (rows apart, gradients asked for): what a pair keeps and returns hangs on no autograd graph."""
+    g = rng(17)
+    def apart(*shape):                                         # rows of a wider tensor, a leaf of its own
+        t = torch.empty_strided(shape, (shape[1] * (shape[2] + 3), shape[2] + 3, 1), device="cuda")
+        return t.copy_(normal(g, *shape)).requires_grad_()
+    u, start, dwin, dy = apart(2, 9, 16), apart(2, 3, 16), apart(2, 3, 16), apart(2, 9, 16)
+    w, b = normal(g, 16, 4).t().contiguous().t().cuda().requires_grad_(), normal(g, 32).cuda()[::2].detach().requires_grad_()
+    y, window, saved = nmpc_amd.causal_conv_fwd(u, w, b, "silu", start)
+    grads = nmpc_amd.causal_conv_bwd(saved, dy, dwin)
+    wg = normal(g, 24, 16).cuda().requires_grad_()
+    h, fsaved = nmpc_amd.gated_ffn_fwd(u, wg, wg)
+    dh = apart(2, 9, 24)
+    fgrads = nmpc_amd.gated_ffn_bwd(fsaved, dh)
+    for t in [y, window, h, *saved.tensors, *fsaved.tensors, *grads.values(), *fgrads]:
+        assert t is None or t.grad_fn is None
+    plain = lambda t: t.detach().contiguous()                  # noqa: E731
+    want = nmpc_amd.causal_conv_bwd(nmpc_amd.causal_conv_fwd(*map(plain, (u, w, b)), "silu", plain(start))[2], plain(dy), plain(dwin))
+    assert all(torch.equal(grads[k], want[k]) for k in want)

@@ -379,6 +379,7 @@ inline int conv_nch(int L, int run) { return L > run ? (L + run - 1) / run : 1; 
 static int conv_check(const char* what, int nb, int L, int D, int W, int act) {
     NMPC_REQUIRE(nb >= 0 && L >= 0 && D >= 1, "%s: bad sizes (%d sequences, %d steps, %d channels)", what, nb, L, D);
     NMPC_REQUIRE(W >= 1 && W <= CONV_MAX_W, "%s: %d taps (1..%d)", what, W, CONV_MAX_W);
+    NMPC_REQUIRE(D < 1 << 30, "%s: %d channels (fewer than 2^30)", what, D);       // the sums of dw: four threads a channel, fewer than 2^32 a launch
     NMPC_REQUIRE(act == NMPC_ACT_NONE || act == NMPC_ACT_SILU, "%s: activation %d (none or silu)", what, act);
     NMPC_REQUIRE(L <= 1 << 30, "%s: at most 2^30 steps", what);
     NMPC_REQUIRE((long long)nb * conv_nch(L, CONV_TR) * D < (1ll << 31), "%s: too many elements for one launch", what);

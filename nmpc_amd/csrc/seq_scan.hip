@@ -1163,6 +1163,8 @@ extern "C" int nmpc_lpv_scan_bwd(const nmpc_scan_args* args, void* stream) {
     NMPC_REQUIRE(a.A && a.dA, "nmpc_lpv_scan_bwd: null argument");
     NMPC_REQUIRE(a.nb == 0 || a.L == 0 || (a.u && a.dt && a.B && a.C && a.saved && a.dy && a.du && a.ddt && a.dB && a.dC && (!a.z || a.dz)),
                  "nmpc_lpv_scan_bwd: null argument");
+    // the sums of the parameters' gradients: four threads a value, fewer than 2^32 a launch
+    NMPC_REQUIRE((long long)a.D * (4 * scan_lanes(a.N) + 2) < 1ll << 30, "nmpc_lpv_scan_bwd: too many channels and states for one launch");
     NMPC_REQUIRE(!a.D_skip || a.dD, "nmpc_lpv_scan_bwd: D needs dD");
     NMPC_REQUIRE(!a.dt_bias || a.ddt_bias, "nmpc_lpv_scan_bwd: dt_bias needs ddt_bias");
     scan_plan(s, true);

@@ -242,3 +242,21 @@ def test_plan_queries():
     for product, most in ((0, (64, 32, 16)), (1, (256, 256, 64)), (2, (256, 256, 64))):       # one row: the kernel for few rows forward
         assert L.nmpc_gated_ffn_plan(1, 1, 2048, 8192, product, 0, at) == 0
         assert all(1 <= v <= top for v, top in zip(shape, most)) and (shape[1] == 32) == (product == 0)
+
+
+def test_sizes_past_one_launch_are_refused_before_anything_runs():
+    """The sums of the parameters' gradients take four threads a value: channels whose sums do not fit a launch are refused at the entry, not
+    by the runtime after the kernels before them."""
+    L = _lib.lib()
+    buf = (ctypes.c_float * 64)()
+    p = ctypes.addressof(buf)
+    many = 1 << 30
+    for nb in (0, 1):
+        assert L.nmpc_causal_conv_bwd(1, nb, 1, many, 1, p, many, many, p, None, 0, None, None, p, many, many, None, p, p, None, None, p, 1 << 62, None) != 0
+        assert b"channels (fewer than 2^30)" in L.nmpc_last_error()
+    s = _lib.ScanArgs()
+    s.struct_size, s.nb, s.L, s.D, s.N, s.G = ctypes.sizeof(s), 1, 1, 1 << 24, 64, 1
+    for k in ("u", "dt", "B", "C", "A", "saved", "dy", "du", "ddt", "dB", "dC", "dA", "workspace"):
+        setattr(s, k, (p + 15) // 16 * 16)
+    s.workspace_bytes = 1 << 62
+    assert L.nmpc_lpv_scan_bwd(ctypes.addressof(s), None) != 0 and b"too many channels and states" in L.nmpc_last_error()

@@ -306,7 +306,9 @@ int nmpc_causal_conv_step(int dtype, int nb, int D, int W, void* window, const v
  * nmpc_lpv_scan_step: one sample of every sequence, u / dt / z [nb][D], B / C [nb][G][N] (_ts unused); `last` is the state,
  * read and replaced.
  * workspace: nmpc_lpv_scan_workspace_bytes (0 for some sizes), contents need not be preserved; calls that overlap in time
- * need one each.  saved and workspace start on 16 bytes.  Strides between steps are 0..2^24 elements. */
+ * need one each.  saved and workspace start on 16 bytes.  Strides between steps are 0..2^24 elements.
+ * Modes may grow (delta A > 0): by less than 2^127 in one step, by any factor over a record. What
+ * leaves fp32's range is infinite. */
 typedef struct nmpc_scan_args {
     int struct_size;                     /* sizeof(nmpc_scan_args) of the caller's header; checked */
     int dtype, nb, L, D, N, G, softplus;

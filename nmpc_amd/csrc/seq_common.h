@@ -24,7 +24,7 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& x) {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// 1 / (1 + e^-x); e^-x overflows to infinity and the reciprocal to 0 where the value is below 2^-126
+// 1 / (1 + e^-x), exponential and reciprocal of one unit in the last place each; e^-x overflows to infinity and the reciprocal to 0 where the value is below 2^-126
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
 
 // steps of sequence b that count: lengths[b] clamped to 0 .. L

@@ -7,9 +7,9 @@
 // operands of the next products, which take both side by side: dx is one product over 2 F, [dWg; dWu] one of 2 F rows.
 // What bounds it: many rows the matrix cores, few rows reading the weights, a prompt of a few hundred rows the latency of its loads.
 // Measured: bf16 4096 x 2048 x 8192 forward 264 us (1.04 PFLOP/s), 340 with both projections kept, gradient 585 us: 0.9 PFLOP/s over
-// training steps, which hold the chip at its power limit (the library's plain products of these sizes reach 1.1 .. 1.3; writing the
-// projections past the caches is 36 us faster alone and no faster in training steps); fp32 4096 x 256 x 1024 training 160 us
-// (81 TFLOP/s); bf16 1 x 2048 x 8192 12.9 us, 5.2 TB/s.
+// training steps, which hold the chip at its power limit (1.83 GHz in both gradients; the library's plain products of these sizes reach
+// 1.1 .. 1.3; writing the projections past the caches is 36 us faster alone and no faster in training steps); fp32 4096 x 256 x 1024
+// training 162 us (80 TFLOP/s); bf16 1 x 2048 x 8192 12.9 us, 5.2 TB/s.
 #include <cmath>
 
 #include "seq_common.h"

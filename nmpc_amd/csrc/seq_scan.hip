@@ -16,7 +16,7 @@
 // 6.5 are the states of a tile computed again from the one saved before it: saving every 16th state costs 1/4 byte a state and step
 // instead of 4.  Sums over the lanes of a channel and over the channels of a group trade
 // halves, so that four steps (eight values) share the stages of one.
-// Measured, bf16, 16 states: 4 x 2048 steps x 2048 channels forward 122 us, training 483 us (279 of them the main backward pass);
+// Measured, bf16, 16 states: 4 x 2048 steps x 2048 channels forward 124 us, training 483 us (280 of them the main backward pass);
 // 1 x 8192 x 2048 forward 152 us; step of 64 x 4096 channels 9.5 us, 3.8 TB/s.
 #include <algorithm>
 #include <cmath>
@@ -198,6 +198,7 @@ struct Shared {
     }
 };
 
+// A log2(e): rounded once more than delta A would be, by half a step of the exponent, which saves a product a state and step
 template <int P>
 __device__ __forceinline__ void load_A(const ScanDev& s, int c, bool ok, int q, float (&a)[4]) {
 #pragma unroll
@@ -1016,7 +1017,7 @@ static void scan_plan(ScanDev& s, bool backward) {
     const double work = (double)a.nb * a.D * a.L * 4 * P * 1e-6;
     const double whole = std::max((backward ? 13.7 : 4.0) * s.ntile, (backward ? 1.03 : 0.35) * work);
     const double slots = backward ? 1e30 : std::max(3.0 * ((a.L + 63) / 64), 0.45 * work);
-    const long long want = (1024 + base - 1) / base;            // chunks that fill the chip: four workgroups a CU
+    const long long want = (1024 + base - 1) / base;            // chunks of 1024 workgroups: four a CU, of which one to three run at once
     double chunks = 1e30;
     int tpc = s.ntile;
     for (long long t = want < s.ntile ? (s.ntile + want - 1) / want : 1; t < s.ntile; t *= 2) {
